@@ -5,51 +5,20 @@
 // mode 1: the loss is the plain negative log likelihood and only the gradient is smoothed, uniformly over all V classes
 //         (q = (1-s) one-hot + s/V): what an identity with a smoothing backward between log-softmax and the loss computes.
 // The forward kernel optionally writes the arg max of each row (first index among equal maxima).
-#include "common.cuh"
+#include "class_rows.cuh"
 #include <type_traits>
 
 namespace {
 
-__device__ __forceinline__ float ld(const void* x, int64_t i, int is_bf16) {
-  return is_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(x)[i]) : reinterpret_cast<const float*>(x)[i];
-}
-
-// A row of an odd vocabulary starts anywhere: single elements up to the first 16-byte boundary of the logits, 16-byte accesses from there
-// on, single elements at the end. (With single elements for every such row, 6000 x 10025 took as long as 6000 x 32000.)
-__device__ __forceinline__ int row_head(const void* x, int64_t base, int v, int elem) {
-  const int off = (int)((reinterpret_cast<uintptr_t>(x) + (uint64_t)base * elem) & 15);
-  return min(off ? (16 - off) / elem : 0, v);
-}
+using rows::Chunk;
+using rows::ld;
+using rows::row_head;
 
 // kArg: the arg max is wanted, kTot: the plain sum of the row is (label smoothing in the loss). Every class costs an exponential, and the
 // instructions around it are what kept the pass from the rate of its reads: with the position of the maximum searched and the sum taken for
 // every caller, 6001 x 32000 bf16 took 89 us (4.3 TB/s). The maximum of a group comes from packed 16-bit comparisons, and its position is
 // looked up only in batches that hold a new one; a batch of 32 classes changes the running maximum once.
 //
-// 16 bytes: 8 bf16 or 4 fp32 values
-template <bool kBf16>
-struct Chunk {
-  static constexpr int kN = kBf16 ? 8 : 4;
-  uint4 u;
-  __device__ __forceinline__ void load(const void* x, int64_t at) {
-    u = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(x) + at * (kBf16 ? 2 : 4));
-  }
-  __device__ __forceinline__ void fill_neg_inf() { u.x = u.y = u.z = u.w = kBf16 ? 0xff80ff80u : 0xff800000u; }
-  __device__ __forceinline__ float at(int i) const {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
-    if (kBf16) return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
-    return __uint_as_float(w[i]);
-  }
-  __device__ __forceinline__ float max() const {
-    if (kBf16) {
-      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-      const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
-      return fmaxf(m.x, m.y);
-    }
-    return fmaxf(fmaxf(at(0), at(1)), fmaxf(at(2), at(3)));
-  }
-};
-
 // kBatch: chunks of a row that a thread has in flight. Two where four would leave half of the last batch of loads empty (up to little more than 4096
 // classes, and from 9000 to 12288), and up to 16383 with the position of the maximum, whose search goes through all chunks; else four. us, bf16, out of memory, four / two:
 // with the sum of the row 6000 x 1000 12.0 / 11.1, x 4000 18.4 / 17.0, x 6000 21.4 / 22.3, x 8000 24.6 / 25.3, x 10001 33.2 / 31.7, x 14000 37.5 / 38.4,
