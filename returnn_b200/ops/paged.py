@@ -24,6 +24,7 @@ import ctypes
 import math
 import torch
 from . import _lib
+from .gemm import status_tensor
 
 __all__ = ["AppendedTokens", "ReleasedPages", "append_tokens", "release_pages", "paged_attention", "append_tokens_reference",
            "release_pages_reference", "paged_attention_reference"]
@@ -181,9 +182,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         out = torch.empty(n, heads, d, dtype=q.dtype, device=q.device)
         # (the stride of an axis of one element is never used)
         st = (_i64 * 8)(q.stride(0), q.stride(1), *(s if m > 1 else 0 for c in (k_cache, v_cache) for s, m in zip(c.stride()[:3], c.shape)))
-        fn = _lib.bind("rb200_paged_attention", [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp])
+        fn = _lib.bind("rb200_paged_attention", [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp])
         _lib.check(fn(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), lengths.data_ptr(), out.data_ptr(),
-                      work.data_ptr(), st, n, heads, kv_heads, d, page, block_table.shape[1], pages, scale, bf16, _lib.stream_ptr()), what)
+                      work.data_ptr(), st, n, heads, kv_heads, d, page, block_table.shape[1], pages, scale, bf16, status_tensor(q.device).data_ptr(), _lib.stream_ptr()), what)
         _lib.count_launch(2)
     return out
 
