@@ -35,6 +35,7 @@ struct Args {
   int* status;
   int64_t q_req, q_head, kp, kh, kt, vp, vh, vt, table_stride;
   int n, heads, kv_heads, d, page, blocks, num_pages, group, units_per_kv, unit_heads, grid;
+  int whole;  // 16 tokens from a multiple of 16 on lie in one page, and rows are as wide as in shared memory
   float scale_log2;
 };
 
@@ -88,6 +89,9 @@ __device__ __forceinline__ void next(const Args& a, Place& p, int units) {
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool real) {  // zeros unless real
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 // this thread's arrival at the barrier, once its copies so far are there
 __device__ __forceinline__ void arrive_copied(uint64_t* bar) {
@@ -413,29 +417,40 @@ attention_kernel(const Args a) {
   bool ok = true;
 
   if (warp >= kWarps) {
-    // ---- loads. Loading warp w has the parts of 16 tokens w, w + kLoaders, ... of a tile; lane r looks the page of row r of a part up, while the tile in
-    // front is waited for
+    // ---- loads. Loading warp w has the parts of 16 tokens w, w + kLoaders, ... of a tile; lane r looks the page of row r of a part up, a tile ahead
     constexpr int kMyParts = kWarps / kLoaders, kPer = 16 / (int)sizeof(T), kCopies = S::kRowBytes / 16;
     static_assert(kMyParts <= 2, "a lane per row");
     const int loader = warp - kWarps, my_row = (loader + (lane >> 4) * kLoaders) * kRows + (lane & 15);
     const bool mine_at_all = (lane >> 4) < kMyParts;
-    Place p = start_shared;
-    int pg = -1;
+    Place p = start_shared, ahead = p;
+    int pg = -1, at = 0, ahead_pg = -1, ahead_at = 0;
     auto look_up = [&]() {
-      const int64_t t = (int64_t)p.tile * S::kTile + my_row;
-      if (mine_at_all && t < p.len) pg = a.table[(int64_t)p.req * a.table_stride + (int)t / a.page];
+      const int64_t t = (int64_t)ahead.tile * S::kTile + my_row;
+      ahead_pg = -1;
+      if (mine_at_all && t < ahead.len) {
+        const int b = (int)t / a.page;
+        ahead_at = (int)t - b * a.page;
+        ahead_pg = a.table[(int64_t)ahead.req * a.table_stride + b];
+      }
     };
     look_up();
+    const int64_t k_step = a.kt * (int64_t)sizeof(T) * (32 / kCopies > 0 ? 32 / kCopies : 1), v_step = a.vt * (int64_t)sizeof(T) * (32 / kCopies > 0 ? 32 / kCopies : 1);
     int n = 0, s = 0, round = 0;
 #pragma unroll 1
     for (; n < n_tiles; ++n) {
-      const int64_t t = (int64_t)p.tile * S::kTile + my_row;
-      const bool real = mine_at_all && t < p.len && pg >= 0 && pg < a.num_pages;  // (a page that is none: as if the token were not there)
+      p = ahead;
+      pg = ahead_pg;
+      at = ahead_at;
+      if (n + 1 < n_tiles) {
+        next<S::kTile>(a, ahead, units);
+        look_up();
+      }
+      const bool real = pg >= 0 && pg < a.num_pages;  // (no such token; or a page that is none: as if the token were not there)
       const uint32_t bits = __ballot_sync(0xffffffffu, real);
-      const int64_t at = real ? (int64_t)((uint32_t)t % (uint32_t)a.page) : 0, in = real ? pg : 0;
-      const int kv = p.unit / a.units_per_kv;
-      const int64_t k_row = (int64_t)a.k + (int64_t)sizeof(T) * (in * a.kp + kv * a.kh + at * a.kt);
-      const int64_t v_row = (int64_t)a.v + (int64_t)sizeof(T) * (in * a.vp + kv * a.vh + at * a.vt);
+      const int64_t place = real ? at : 0, in = real ? pg : 0;
+      const int kv = a.units_per_kv == 1 ? p.unit : p.unit / a.units_per_kv;
+      const int64_t k_row = (int64_t)a.k + (int64_t)sizeof(T) * (in * a.kp + kv * a.kh + place * a.kt);
+      const int64_t v_row = (int64_t)a.v + (int64_t)sizeof(T) * (in * a.vp + kv * a.vh + place * a.vt);
 #pragma unroll
       for (int j = 0; j < kMyParts; ++j) {
         const int part = loader + j * kLoaders;
@@ -443,6 +458,20 @@ attention_kernel(const Args a) {
         if (!ok) break;
         const uint32_t to = smem_u32(smem) + s * S::kStage + part * S::kPart;
         const uint32_t mine = bits >> (16 * j);
+        if (kCopies <= 32 && a.whole && (mine & 0xffffu) == 0xffffu) {  // 16 tokens of one page: rows at a fixed distance
+          const int row0 = lane / kCopies, c = lane % kCopies;
+          int64_t kr = __shfl_sync(0xffffffffu, k_row, 16 * j) + row0 * a.kt * (int64_t)sizeof(T) + c * 16;
+          int64_t vr = __shfl_sync(0xffffffffu, v_row, 16 * j) + row0 * a.vt * (int64_t)sizeof(T) + c * 16;
+#pragma unroll
+          for (int i = 0; i < kRows * kCopies / 32; ++i) {
+            const int row = i * (32 / kCopies) + row0;
+            const uint32_t dst = to + (c >> 3) * (kRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+            copy16(dst, reinterpret_cast<const void*>(kr));
+            copy16(dst + kWarps * S::kPart, reinterpret_cast<const void*>(vr));
+            kr += k_step;
+            vr += v_step;
+          }
+        } else {
 #pragma unroll
         for (int i = 0; i < kRows * kCopies / 32; ++i) {
           const int id = i * 32 + lane, row = id / kCopies, c = id % kCopies;
@@ -452,12 +481,13 @@ attention_kernel(const Args a) {
           copy16(dst, reinterpret_cast<const void*>(kr + (there ? c * 16 : 0)), there);
           copy16(dst + kWarps * S::kPart, reinterpret_cast<const void*>(vr + (there ? c * 16 : 0)), there);
         }
+        }
         arrive_copied(&full[s][part]);
         if (lane == 0) {
           const int64_t t0 = (int64_t)p.tile * S::kTile + part * kRows;
           Note& note = notes[s][part];
           note.word = (mine & 0xffffu) | (t0 < p.len ? 1u << 16 : 0u) | (p.tile + 1 == p.tiles ? 1u << 17 : 0u);
-          note.p = p;
+          if (p.tile == 0 || n == 0) note.p = p;  // (read where outputs begin)
           arrive(&full[s][part]);
         }
       }
@@ -466,8 +496,6 @@ attention_kernel(const Args a) {
         s = 0;
         ++round;
       }
-      next<S::kTile>(a, p, units);
-      if (n + 1 < n_tiles) look_up();
     }
     if (!ok) {  // a wait ran out
       *abort = 1;
@@ -618,8 +646,9 @@ join_kernel(const Args a, int units) {
 }
 
 template <typename T, int DP, int MT>
-int launch(const Args& a, cudaStream_t stream) {
+int launch(Args a, cudaStream_t stream) {
   using S = Shape<T, DP>;
+  a.whole = a.page % kRows == 0 && a.d == DP;
   static_assert(S::kStages >= 2 && S::kSmem + 1536 <= 227 * 1024, "shared memory");
   static RbPerDevice ready;
   auto kernel = attention_kernel<T, DP, MT>;
