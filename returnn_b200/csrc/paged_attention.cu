@@ -2,8 +2,8 @@
 //   out[i, h, :] = softmax_t(scale q[i, h, :] . K[t, h / G, :]) V[t, h / G, :],  t < len_i; token t lies in page table[i][t / P] at place t % P
 // G = query heads per key head. A request without tokens gets zeros. Every key and value is read once; the pass is bound by that.
 //
-// Split: the work is a list of tiles of tokens, ordered by (request, unit of heads, tile); each CTA takes an equal stretch of the list, whatever
-// the lengths of the requests are (a long document next to short ones, few requests of many tokens). A stretch that holds all tiles of a (request, unit)
+// Split: the work is a list of tiles of tokens, ordered by (request, unit of heads, tile); each CTA takes an equally costly stretch of the list, whatever
+// the lengths of the requests are (a long document next to short ones, few requests of many tokens); a (request, unit) costs as much as two tiles more than it has. A stretch that holds all tiles of a (request, unit)
 // writes the result; one that holds some of them leaves its maximum, sum and unnormalised output in 32 bits, and a second small kernel joins those.
 // A unit is a key head with up to 8 * MT of its query heads.
 //
@@ -35,6 +35,7 @@ struct Args {
   int* status;
   int64_t q_req, q_head, kp, kh, kt, vp, vh, vt, table_stride;
   int n, heads, kv_heads, d, page, blocks, num_pages, group, units_per_kv, unit_heads, grid;
+  int q_words;  // queries can be read two features at a time
   int whole;  // 16 tokens from a multiple of 16 on lie in one page, and rows are as wide as in shared memory
   float scale_log2;
 };
@@ -58,28 +59,24 @@ struct Shape {
 };
 
 struct Place {  // in the list of tiles
-  int req, unit, tile, tiles, len;
+  int req, unit, tile, tiles, len;  // tiles: of the request
 };
 
-// What a loading warp says of 16 tokens. word: the tokens that there are as bits; bit 16: some lie within the length; bit 17: the last tile of its (request, unit)
-struct Note {
-  uint32_t word;
-  Place p;
-};
+constexpr int kUnitCost = 2;  // of beginning and ending a (request, unit), in tiles: queries, the meeting of the warps, the result
 
 __device__ __forceinline__ int length_of(const Args& a, int req) { return (int)min((int64_t)max(a.lens[req], 0), (int64_t)a.blocks * a.page); }
 template <int kTile>
 __device__ __forceinline__ int tiles_of(int len) { return (int)(((int64_t)len + kTile - 1) / kTile); }
 
+// first tile of the next (request, unit)
 template <int kTile>
-__device__ __forceinline__ void next(const Args& a, Place& p, int units) {
-  if (++p.tile < p.tiles) return;
+__device__ __forceinline__ void next_unit(const Args& a, Place& p, int units) {
   p.tile = 0;
   if (++p.unit < units) return;
   p.unit = 0;
   do {
     if (++p.req >= a.n) {
-      p.tiles = 0;
+      p.tiles = p.len = 0;
       return;
     }
     p.len = length_of(a, p.req);
@@ -130,7 +127,7 @@ struct State<__nv_bfloat16, DP> {
   float o[kTiles][4];
   float m, l;  // l: of this lane's columns
 
-  __device__ __forceinline__ void begin(const Args& a, const Place& p, int m_tile) {
+  __device__ __forceinline__ void fetch_queries(const Args& a, const Place& p, int m_tile) {
     const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
     const int kv = p.unit / a.units_per_kv, h = (p.unit % a.units_per_kv) * a.unit_heads + m_tile * 8 + g;
     const bool real = h < a.group && m_tile * 8 + g < a.unit_heads;
@@ -140,9 +137,15 @@ struct State<__nv_bfloat16, DP> {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const int e = s * 16 + b * 8 + j * 2;
-        const uint16_t* u = reinterpret_cast<const uint16_t*>(src);
-        q[s][b] = real && e < a.d ? (uint32_t)u[e] | (uint32_t)u[e + 1] << 16 : 0u;  // (D is a multiple of 8)
+        uint32_t x = 0u;
+        if (real && e < a.d) {  // (D is a multiple of 8)
+          const uint16_t* u = reinterpret_cast<const uint16_t*>(src) + e;
+          x = a.q_words ? *reinterpret_cast<const uint32_t*>(u) : (uint32_t)u[0] | (uint32_t)u[1] << 16;
+        }
+        q[s][b] = x;
       }
+  }
+  __device__ __forceinline__ void begin() {
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     m = -INFINITY;
@@ -257,7 +260,7 @@ struct State<float, DP> {
                   ? reinterpret_cast<const float*>(a.q)[p.req * a.q_req + (int64_t)(kv * a.group + h0 + g) * a.q_head + e] * a.scale_log2 : 0.f;
     }
   }
-  __device__ __forceinline__ void begin(const Args&, const Place&, int) {
+  __device__ __forceinline__ void begin() {
 #pragma unroll
     for (int g = 0; g < 8; ++g) {
       m[g] = -INFINITY;
@@ -359,8 +362,8 @@ attention_kernel(const Args a) {
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   float* boxes = reinterpret_cast<float*>(smem + kStages * S::kStage);
   __shared__ uint64_t full[kStages][kWarps], empty[kStages][kWarps], meeting;
-  __shared__ Note notes[kStages][kWarps];
-  __shared__ long long warp_sums[kWarps + kLoaders];
+  __shared__ uint32_t notes[kStages][kWarps];  // of 16 tokens: those that there are as bits; bit 16: some lie within the length
+  __shared__ long long warp_sums[kWarps + kLoaders][2], rank_shared[2], cost_shared;
   __shared__ Place start_shared;
   __shared__ int abort_shared;
   volatile int* abort = &abort_shared;
@@ -378,42 +381,67 @@ attention_kernel(const Args a) {
   rb_pdl_wait();
   rb_pdl_launch();
 
-  // this CTA's stretch of the list: prefix sums over the requests, a run of them per thread
+  // This CTA's stretch of the list: prefix sums of cost and tiles over the requests, a run of them per thread. A place in the list is a cost; those that fall to the
+  // beginning of a (request, unit) stand for its first tile.
   const int run = (a.n + (int)blockDim.x - 1) / (int)blockDim.x;
   const int r0 = min((int64_t)a.n, (int64_t)threadIdx.x * run), r1 = min(a.n, r0 + run);
-  long long mine = 0;
-  for (int r = r0; r < r1; ++r) mine += (long long)tiles_of<S::kTile>(length_of(a, r)) * units;
-  long long inc = mine;
+  auto cost_of = [&](int tiles) { return tiles ? (long long)(tiles + kUnitCost) * units : 0LL; };
+  long long mine = 0, mine_tiles = 0;
+  for (int r = r0; r < r1; ++r) {
+    const int tiles = tiles_of<S::kTile>(length_of(a, r));
+    mine += cost_of(tiles);
+    mine_tiles += (long long)tiles * units;
+  }
+  long long inc = mine, inc_tiles = mine_tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += x;
+    const long long x = __shfl_up_sync(0xffffffffu, inc, o), y = __shfl_up_sync(0xffffffffu, inc_tiles, o);
+    if (lane >= o) {
+      inc += x;
+      inc_tiles += y;
+    }
   }
-  if (lane == 31) warp_sums[warp] = inc;
+  if (lane == 31) {
+    warp_sums[warp][0] = inc;
+    warp_sums[warp][1] = inc_tiles;
+  }
   __syncthreads();
-  long long total = 0, before = inc - mine;
+  long long total = 0, total_tiles = 0, before = inc - mine, before_tiles = inc_tiles - mine_tiles;
 #pragma unroll
   for (int w = 0; w < kWarps + kLoaders; ++w) {
-    if (w < warp) before += warp_sums[w];
-    total += warp_sums[w];
+    if (w < warp) {
+      before += warp_sums[w][0];
+      before_tiles += warp_sums[w][1];
+    }
+    total += warp_sums[w][0];
+    total_tiles += warp_sums[w][1];
   }
   const long long per = max((total + a.grid - 1) / a.grid, 1LL);
   const long long first = per * blockIdx.x, last = min(total, first + per);
   if (first >= last) return;
-  if (before <= first && first < before + mine) {
+  if (threadIdx.x == 0 && last == total) rank_shared[1] = total_tiles;
+  for (int end = 0; end < 2; ++end) {
+    const long long want = end ? last : first;
+    if (!(before <= want && want < before + mine)) continue;
+    long long c = before, k = before_tiles;
     for (int r = r0; r < r1; ++r) {
       const int len = length_of(a, r), tiles = tiles_of<S::kTile>(len);
-      const long long all = (long long)tiles * units;
-      if (first < before + all) {
-        const long long in = first - before;
-        start_shared = Place{r, (int)(in / tiles), (int)(in % tiles), tiles, len};
+      if (want < c + cost_of(tiles)) {
+        const long long in = want - c;
+        const int unit = (int)(in / (tiles + kUnitCost)), tile = max((int)(in % (tiles + kUnitCost)) - kUnitCost, 0);
+        rank_shared[end] = k + (long long)unit * tiles + tile;
+        if (!end) {
+          start_shared = Place{r, unit, tile, tiles, len};
+          cost_shared = c + (long long)unit * (tiles + kUnitCost);
+        }
         break;
       }
-      before += all;
+      c += cost_of(tiles);
+      k += (long long)tiles * units;
     }
   }
   __syncthreads();
-  const int n_tiles = (int)(last - first);
+  const int n_tiles = (int)(rank_shared[1] - rank_shared[0]);
   bool ok = true;
 
   if (warp >= kWarps) {
@@ -442,7 +470,7 @@ attention_kernel(const Args a) {
       pg = ahead_pg;
       at = ahead_at;
       if (n + 1 < n_tiles) {
-        next<S::kTile>(a, ahead, units);
+        if (++ahead.tile == ahead.tiles) next_unit<S::kTile>(a, ahead, units);
         look_up();
       }
       const bool real = pg >= 0 && pg < a.num_pages;  // (no such token; or a page that is none: as if the token were not there)
@@ -485,9 +513,7 @@ attention_kernel(const Args a) {
         arrive_copied(&full[s][part]);
         if (lane == 0) {
           const int64_t t0 = (int64_t)p.tile * S::kTile + part * kRows;
-          Note& note = notes[s][part];
-          note.word = (mine & 0xffffu) | (t0 < p.len ? 1u << 16 : 0u) | (p.tile + 1 == p.tiles ? 1u << 17 : 0u);
-          if (p.tile == 0 || n == 0) note.p = p;  // (read where outputs begin)
+          notes[s][part] = (mine & 0xffffu) | (t0 < p.len ? 1u << 16 : 0u);
           arrive(&full[s][part]);
         }
       }
@@ -517,46 +543,48 @@ attention_kernel(const Args a) {
     ok = warp_wait(&meeting, meetings++ & 1, abort);
   };
   State<T, DP> st;
-  Place cur = start_shared;  // the tile at which this warp's present outputs began
-  bool fresh = true;
-  long long g0 = 0;  // number of the first tile of the (request, unit) in the list
+  Place cur = start_shared;
+  long long cost = cost_shared;  // where the present (request, unit) begins
+  if constexpr (S::kBf16) st.fetch_queries(a, cur, m_tile);
   int n = 0, s = 0, round = 0;
 #pragma unroll 1
-  for (; n < n_tiles; ++n) {
-    constexpr int kMine = kWarps / kShares;  // parts of 16 tokens that are this warp's
-    bool ends = false;
-#pragma unroll 1
-    for (int i = 0; i < kMine; ++i) {
-      const int w = share * kMine + i;
-      ok = warp_wait(&full[s][w], round & 1, abort);
+  while (n < n_tiles) {
+    const int count = min(cur.tiles - cur.tile, n_tiles - n);
+    if constexpr (!S::kBf16) {
+      st.share_queries(a, cur, qs);
+      meet();
       if (!ok) break;
-      const uint32_t word = notes[s][w].word;
-      ends = word >> 17 & 1;
-      if (fresh) {
-        cur = notes[s][w].p;
-        if constexpr (!S::kBf16) {
-          st.share_queries(a, cur, qs);
-          meet();
-          if (!ok) break;
+    }
+    st.begin();
+#pragma unroll 1
+    for (int t = 0; t < count && ok; ++t) {
+      constexpr int kMine = kWarps / kShares;  // parts of 16 tokens that are this warp's
+#pragma unroll 1
+      for (int i = 0; i < kMine; ++i) {
+        const int w = share * kMine + i;
+        ok = warp_wait(&full[s][w], round & 1, abort);
+        if (!ok) break;
+        const uint32_t word = notes[s][w];
+        if (word >> 16) {
+          const uint32_t keys = stages + s * S::kStage + w * S::kPart;
+          st.add(a, keys, keys + kWarps * S::kPart, word & 0xffffu, qs, ps);
         }
-        st.begin(a, cur, m_tile);
-        g0 = first + n - cur.tile;
-        fresh = false;
+        __syncwarp();
+        if (lane == 0) arrive(&empty[s][w]);
       }
-      if (word >> 16 & 1) {
-        const uint32_t keys = stages + s * S::kStage + w * S::kPart;
-        st.add(a, keys, keys + kWarps * S::kPart, word & 0xffffu, qs, ps);
+      if (++s == kStages) {
+        s = 0;
+        ++round;
       }
-      __syncwarp();
-      if (lane == 0) arrive(&empty[s][w]);
     }
     if (!ok) break;
-    if (++s == kStages) {
-      s = 0;
-      ++round;
+    n += count;
+    const Place done = cur;
+    const bool ends = cur.tile + count == cur.tiles, whole = cur.tile == 0;
+    if (n < n_tiles) {  // the next queries are under way while the warps meet
+      next_unit<S::kTile>(a, cur, units);
+      if constexpr (S::kBf16) st.fetch_queries(a, cur, m_tile);
     }
-    if (!ends && n + 1 < n_tiles) continue;
-    const bool whole = cur.tile == 0;
     // ---- the warps' outputs come together
     st.finish();
     if constexpr (S::kBf16) {
@@ -566,7 +594,7 @@ attention_kernel(const Args a) {
     st.give(boxes + warp * S::kMeet);
     meet();
     if (!ok) break;
-    const int kv = cur.unit / a.units_per_kv, h0 = (cur.unit % a.units_per_kv) * a.unit_heads;
+    const int kv = done.unit / a.units_per_kv, h0 = (done.unit % a.units_per_kv) * a.unit_heads;
     for (int i = threadIdx.x; i < 8 * MT * (DP / 4); i += kWarps * 32) {
       const int e = i % (DP / 4) * 4, g = i / (DP / 4) % 8, mt = i / (DP / 4) / 8, h = mt * 8 + g;
       if (e >= a.d || h >= a.unit_heads || h0 + h >= a.group) continue;
@@ -587,7 +615,7 @@ attention_kernel(const Args a) {
       }
       if (ends && whole) {
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-        put4(reinterpret_cast<T*>(a.out) + ((int64_t)cur.req * a.heads + kv * a.group + h0 + h) * a.d + e, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        put4(reinterpret_cast<T*>(a.out) + ((int64_t)done.req * a.heads + kv * a.group + h0 + h) * a.d + e, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
       } else {
         float* to = a.part + (((int64_t)blockIdx.x * 2 + (whole ? 1 : 0)) * a.unit_heads + h) * (a.d + 4);
         *reinterpret_cast<float4*>(to + e) = o;
@@ -595,8 +623,8 @@ attention_kernel(const Args a) {
       }
     }
     if (whole && threadIdx.x == 0)
-      a.owners[(int64_t)cur.req * units + cur.unit] = make_int2((int)blockIdx.x, ends ? (int)blockIdx.x : (int)((g0 + cur.tiles - 1) / per));
-    fresh = true;
+      a.owners[(int64_t)done.req * units + done.unit] = make_int2((int)blockIdx.x, ends ? (int)blockIdx.x : (int)((cost + kUnitCost + done.tiles - 1) / per));
+    cost += done.tiles + kUnitCost;
   }
   if (!ok) {
     *abort = 1;
@@ -704,6 +732,7 @@ RB_EXPORT int rb200_paged_attention(const void* q, const void* k, const void* v,
   }
   Args a = {};
   a.q = q; a.k = k; a.v = v; a.table = table; a.lens = lens; a.out = out; a.table_stride = table_stride; a.status = status;
+  a.q_words = (reinterpret_cast<uintptr_t>(q) & 3) == 0 && strides[0] % 2 == 0 && strides[1] % 2 == 0;
   a.q_req = strides[0]; a.q_head = strides[1]; a.kp = strides[2]; a.kh = strides[3]; a.kt = strides[4]; a.vp = strides[5]; a.vh = strides[6]; a.vt = strides[7];
   a.n = n; a.heads = heads; a.kv_heads = kv_heads; a.d = d; a.page = page; a.blocks = blocks; a.num_pages = num_pages; a.group = heads / kv_heads;
   a.units_per_kv = units_of(a.group, bf16, &a.unit_heads);
