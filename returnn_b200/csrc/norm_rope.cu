@@ -7,40 +7,56 @@
 // The angle of a far position does not fit the 24 bits of a float (position 100000 would be off by 0.004 of a radian): p f / (2 pi) is taken in 64
 // bits, its whole turns dropped, and the sine and cosine of the rest taken in 32. One pair of them per (token, pair of features) serves all heads,
 // so a CTA owns whole tokens and keeps the table of its tokens in shared memory.
-// Rows are read once and written once. A row of D features sits in the next power of two of D / 8 lanes, 8 features (16 bytes of bf16) a lane: the mean
-// is a few shuffles, pairs (2i, 2i + 1) are a lane's own, pairs (i, i + R / 2) one shuffle away. Head dims, rotated parts and alignments that do
-// not fit this take a warp per row with single elements.
-#include "common.cuh"
+// Rows are read once and written once. A row of D features sits in the next power of two of D / 8 lanes, 8 features a lane, chosen so that both features of a pair
+// are the lane's own: 8 in a row for pairs (2i, 2i + 1), 4 of each half for pairs (i, i + R / 2). The mean is a few shuffles. Head dims, rotated parts and
+// alignments that do not fit this take a warp per row with single elements.
+// What bounds it is the instructions around 16 bytes: each turn of a warp has addresses that only go on by a fixed step.
+#include "packed_f32.cuh"
 #include <algorithm>
+#include <cstdlib>
 #include <initializer_list>
+#include <type_traits>
 
 namespace {
 
 constexpr int kMaxDim = 256;
 constexpr int kThreads = 256;
+constexpr int kTurnsBf16 = 4, kTurnsF32 = 2, kBackBf16 = 2, kBackF32 = 1;  // rows of a group that are under way at a time, forward and backward
+constexpr int kBackCtas = 4;                                               // of an SM
 
-struct Args {
-  const void *q, *k, *v;            // forward: inputs. backward: x of the norm (null without one)
-  const void *dq, *dk;              // backward: incoming gradients
-  void *out_q, *out_k;              // [N, Hq, D], [N, Hk, D]
-  void *cache_k, *cache_v;          // cache form: where k and v go
-  const void *positions;            // [num_pos], token t has number t % num_pos
-  const float* freq;                // [R / 2]
-  const void *wq, *wk;              // [D] or null
-  float* part;                      // backward: [gridDim.x][2][D] partial sums of dw
-  const int* slots;
-  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, dq_tok, dq_head, dk_tok, dk_head;
-  int64_t ck_page, ck_head, ck_tok, cv_page, cv_head, cv_tok;
-  int64_t num_slots, num_pos;
-  int64_t n;
-  int hq, hk, d, rot, page, pos64, w_bf16, interleaved, tokens_per_cta;
-  float eps, amp;
+struct Rows {        // of queries, keys or values
+  const void* x;     // input; backward: of the norm (null without one)
+  const void* dz;    // backward: incoming gradient
+  const void* w;     // [D] scale or null
+  void* out;         // [N, heads, D] or the cache
+  int64_t tok, head, dz_tok, dz_head;  // strides in elements
+  int64_t page, page_head, page_tok;   // of the cache
+  int heads;
 };
 
-__device__ __forceinline__ float2 turn_of(const Args& a, int64_t token, int i) {
+struct Args {
+  Rows r[3];                        // queries, keys, values (cache form)
+  const void* positions;            // [num_pos], token t has number t % num_pos
+  const float* freq;                // [R / 2]
+  float* part;                      // backward: [gridDim.x][2][D] partial sums of dw
+  const int* slots;
+  int64_t num_slots, num_pos;
+  int64_t n;
+  int d, rot, page, pos64, w_bf16, interleaved;
+  int tokens;                       // of a CTA's tile
+  int step_tk, step_h;              // of a row of a tile: tokens and heads to the next of its group
+  uint32_t rows_inverse, half_inverse;
+  float eps, amp, inv_d;
+};
+
+__device__ __forceinline__ int64_t position_of(const Args& a, int64_t token) {
   if (a.num_pos < a.n) token %= a.num_pos;
-  const int64_t p = a.pos64 ? reinterpret_cast<const long long*>(a.positions)[token] : reinterpret_cast<const int*>(a.positions)[token];
-  double t = (double)p * (double)a.freq[i] * 0.15915494309189533577;  // turns
+  return a.pos64 ? reinterpret_cast<const long long*>(a.positions)[token] : reinterpret_cast<const int*>(a.positions)[token];
+}
+// turns per position
+__device__ __forceinline__ double turns_of(const Args& a, int i) { return (double)a.freq[i] * 0.15915494309189533577; }
+__device__ __forceinline__ float2 turn_of(const Args& a, int64_t position, double turns) {
+  double t = (double)position * turns;
   t -= rint(t);
   float s, c;
   sincospif((float)(2.0 * t), &s, &c);
@@ -56,195 +72,339 @@ __device__ __forceinline__ void put(void* x, int64_t i, float v) { reinterpret_c
 template <typename T>
 constexpr int is_bf16() { return sizeof(T) == 2; }
 
-// where row `head` of `token` goes in the cache form; -1: nowhere (a token without a slot)
-__device__ __forceinline__ int64_t cache_at(const Args& a, int64_t token, int head, int64_t page_stride, int64_t head_stride, int64_t tok_stride) {
+// where a token's place in the cache starts; -1: nowhere (a token without a slot)
+__device__ __forceinline__ int64_t cache_at(const Args& a, const Rows& r, int64_t token) {
   const int64_t slot = a.slots[token];
   if (slot < 0 || slot >= a.num_slots) return -1;
-  const int64_t pg = slot / a.page;
-  return pg * page_stride + head * head_stride + (slot - pg * a.page) * tok_stride;
-}
-
-// the 8 features of this lane turned by the token's angles (sign -1: back)
-template <bool kInter>
-__device__ __forceinline__ void rotate8(F8& x, const float2* tab, int sub, int rot, float sign) {
-  const int e0 = sub * 8;
-  if (kInter) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (e0 + 2 * j < rot) {
-        const float2 t = tab[(e0 >> 1) + j];
-        const float p = x.v[2 * j], r = x.v[2 * j + 1], s = t.y * sign;
-        x.v[2 * j] = p * t.x - r * s;
-        x.v[2 * j + 1] = p * s + r * t.x;
-      }
-    }
-  } else {
-    const int half = rot >> 1, step = half >> 3;  // half is a multiple of 8 here
-    const bool first = e0 < half, in = e0 < rot;
-    const int lane = threadIdx.x & 31;
-    const int src = in ? (first ? lane + step : lane - step) : lane;
-    const float s = first ? -sign : sign;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float other = __shfl_sync(0xffffffffu, x.v[j], src);
-      if (in) {
-        const float2 t = tab[(first ? e0 : e0 - half) + j];
-        x.v[j] = x.v[j] * t.x + other * t.y * s;
-      }
-    }
-  }
+  const int pg = (int)(slot / a.page);
+  return pg * r.page + (slot - (int64_t)pg * a.page) * r.page_tok;
 }
 
 __device__ __forceinline__ float group_sum(float v, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float squares(const F8& x) {
-  float s = 0.f;
+struct P4 {  // 8 numbers in pairs
+  uint64_t v[4];
+};
+__device__ __forceinline__ P4 pairs(const F8& x) { return P4{{two(x.v[0], x.v[1]), two(x.v[2], x.v[3]), two(x.v[4], x.v[5]), two(x.v[6], x.v[7])}}; }
+__device__ __forceinline__ F8 single(const P4& x) {
+  F8 r;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) s += x.v[j] * x.v[j];
-  return s;
+  for (int j = 0; j < 4; ++j) split(x.v[j], r.v[2 * j], r.v[2 * j + 1]);
+  return r;
+}
+__device__ __forceinline__ P4 scaled(const P4& x, float f) {
+  const uint64_t g = two(f, f);
+  return P4{{mul2(x.v[0], g), mul2(x.v[1], g), mul2(x.v[2], g), mul2(x.v[3], g)}};
+}
+__device__ __forceinline__ P4 product(const P4& x, const P4& y) {
+  return P4{{mul2(x.v[0], y.v[0]), mul2(x.v[1], y.v[1]), mul2(x.v[2], y.v[2]), mul2(x.v[3], y.v[3])}};
+}
+__device__ __forceinline__ float dot_of(const P4& x, const P4& y) {
+  uint64_t s = mul2(x.v[0], y.v[0]);
+#pragma unroll
+  for (int j = 1; j < 4; ++j) s = fma2(x.v[j], y.v[j], s);
+  float a, b;
+  split(s, a, b);
+  return a + b;
+}
+// eight scales from shared memory
+__device__ __forceinline__ P4 scales_at(const float* p) {
+  const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(p), b = *reinterpret_cast<const ulonglong2*>(p + 4);
+  return P4{{a.x, a.y, b.x, b.y}};
 }
 
-template <typename T, bool kInter, bool kCache>
-__global__ void __launch_bounds__(kThreads)
-forward_kernel(const Args a, int lanes) {
-  extern __shared__ float2 table[];  // [tokens_per_cta][R / 2]
-  rb_pdl_wait();
-  rb_pdl_launch();
-  const int64_t t0 = (int64_t)blockIdx.x * a.tokens_per_cta;
-  const int nt = (int)min((int64_t)a.tokens_per_cta, a.n - t0);
-  const int half = a.rot >> 1;
-  for (int i = threadIdx.x; i < nt * half; i += kThreads) table[i] = turn_of(a, t0 + i / half, i % half);
-  __syncthreads();
-  const int sub = threadIdx.x & (lanes - 1);
-  const bool real = sub * 8 < a.d;
-  const bool norm = a.wq != nullptr;
-  F8 wq, wk;
-  if (norm && real) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      wq.v[j] = weight_at(a.wq, sub * 8 + j, a.w_bf16);
-      wk.v[j] = weight_at(a.wk, sub * 8 + j, a.w_bf16);
+// A lane's 8 features as they lie in memory: 8 in a row, or twice 4 (kInter false)
+template <typename T, bool kInter>
+struct Raw8;
+template <bool kInter>
+struct Raw8<__nv_bfloat16, kInter> {
+  uint4 u;
+  __device__ __forceinline__ void load(const char* p, int gap) {
+    if (kInter) {
+      u = *reinterpret_cast<const uint4*>(p);
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(p), y = *reinterpret_cast<const uint2*>(p + gap);
+      u = make_uint4(x.x, x.y, y.x, y.y);
     }
   }
-  const int rows = a.hq + a.hk + (kCache ? a.hk : 0);
-  const int groups = kThreads / lanes;
-  const int total = nt * rows;
-  // (all lanes of a warp go round together: the shuffles want them)
-  for (int r0 = blockIdx.y * groups; r0 < total; r0 += gridDim.y * groups) {
-    const int r = r0 + threadIdx.x / lanes;
-    const bool live = r < total && real;
-    const int tk = live ? r / rows : 0;
-    const int h = live ? r - tk * rows : 0;
-    const int64_t token = t0 + tk;
-    F8 x = {};
-    if (live) {
-      if (h < a.hq) x = load8(a.q, token * a.q_tok + h * a.q_head + sub * 8, is_bf16<T>());
-      else if (h < a.hq + a.hk) x = load8(a.k, token * a.k_tok + (h - a.hq) * a.k_head + sub * 8, is_bf16<T>());
-      else x = load8(a.v, token * a.v_tok + (h - a.hq - a.hk) * a.v_head + sub * 8, is_bf16<T>());
-    }
-    const bool value = kCache && h >= a.hq + a.hk;
-    if (norm) {
-      const float inv = rsqrtf(group_sum(squares(x), lanes) / a.d + a.eps);
-      if (live && !value) {
+  __device__ __forceinline__ F8 get() const {
+    F8 r;
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x.v[j] *= inv * (h < a.hq ? wq.v[j] : wk.v[j]);
-      }
+    for (int i = 0; i < 4; ++i) {
+      r.v[2 * i] = __uint_as_float(w[i] << 16);
+      r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
-    F8 y = x;
-    rotate8<kInter>(y, table + tk * half, sub, a.rot, 1.f);
-    if (!live) continue;
-    if (h < a.hq) {
-      store8(a.out_q, (token * a.hq + h) * a.d + sub * 8, y, is_bf16<T>());
-    } else if (!kCache) {
-      store8(a.out_k, (token * a.hk + h - a.hq) * a.d + sub * 8, y, is_bf16<T>());
-    } else if (!value) {
-      const int64_t at = cache_at(a, token, h - a.hq, a.ck_page, a.ck_head, a.ck_tok);
-      if (at >= 0) store8(a.cache_k, at + sub * 8, y, is_bf16<T>());
+    return r;
+  }
+  __device__ __forceinline__ static void store(char* p, int gap, const F8& f) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f.v[2 * i], f.v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    if (kInter) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-      const int64_t at = cache_at(a, token, h - a.hq - a.hk, a.cv_page, a.cv_head, a.cv_tok);
-      if (at >= 0) store8(a.cache_v, at + sub * 8, x, is_bf16<T>());
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(p + gap) = make_uint2(w[2], w[3]);
+    }
+  }
+};
+template <bool kInter>
+struct Raw8<float, kInter> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const char* p, int gap) {
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + gap);
+  }
+  __device__ __forceinline__ F8 get() const { return F8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}}; }
+  __device__ __forceinline__ static void store(char* p, int gap, const F8& f) {
+    *reinterpret_cast<float4*>(p) = make_float4(f.v[0], f.v[1], f.v[2], f.v[3]);
+    *reinterpret_cast<float4*>(p + gap) = make_float4(f.v[4], f.v[5], f.v[6], f.v[7]);
+  }
+};
+
+// What a lane is: features `at` .. + 3 and `at + gap` .. + 3 of the rows of its group; rotated: its pairs are 4 `sub` .. + 3 of the table
+struct Lane {
+  int sub, at, gap, group;
+  bool real, turned;
+};
+template <bool kInter, int kLanes>
+__device__ __forceinline__ Lane lane_of(const Args& a) {
+  Lane l;
+  const int lane = threadIdx.x & 31;
+  l.sub = lane & (kLanes - 1);
+  l.group = lane / kLanes;
+  l.real = l.sub * 8 < a.d;
+  l.turned = l.sub * 8 < a.rot;
+  l.at = l.sub * 8;
+  l.gap = 4;
+  if (!kInter && l.turned) {
+    l.at = l.sub * 4;
+    l.gap = a.rot >> 1;
+  }
+  return l;
+}
+
+// the four pairs of a lane turned (sign -1: back)
+template <bool kInter>
+__device__ __forceinline__ void rotate4(F8& x, const float2* table, const Lane& l, float sign) {
+  if (!l.turned) return;
+  const float4* t = reinterpret_cast<const float4*>(table + l.sub * 4);
+  const float4 t0 = t[0], t1 = t[1];
+  const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y * sign, t0.w * sign, t1.y * sign, t1.w * sign};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float &p = x.v[kInter ? 2 * j : j], &q = x.v[kInter ? 2 * j + 1 : 4 + j];
+    const float u = p * c[j] - q * s[j];
+    q = p * s[j] + q * c[j];
+    p = u;
+  }
+}
+
+// A CTA has the rows (token, head) of a few tokens, queries' heads before keys' and values', a row per group of kLanes lanes and turn. Rows go on by whole steps, so that token
+// and head cost no division; offsets within a tile of tokens are 32 bits wide (see fits).
+struct Walk {
+  int tk, h;
+  __device__ __forceinline__ Walk(int start, uint32_t inverse, int of) {  // inverse: 2^32 / of, rounded up; start below 2^16
+    tk = of == 1 ? start : (int)__umulhi((uint32_t)start, inverse);
+    h = start - tk * of;
+  }
+  __device__ __forceinline__ void go(const Args& a, int of) {
+    tk += a.step_tk;
+    h += a.step_h;
+    if (h >= of) {
+      h -= of;
+      ++tk;
+    }
+  }
+};
+
+// shared memory: the scales of queries and keys in fp32 in the lanes' order, [2][kLanes * 8]; then the angles of the tile's tokens, [tokens][R / 2]
+template <bool kInter, int kLanes>
+__device__ __forceinline__ void fill_scales(const Args& a, float* scales) {
+  if (!a.r[0].w) return;
+  for (int i = threadIdx.x; i < 2 * kLanes * 8; i += kThreads) {
+    const int e = i % (kLanes * 8), sub = e >> 3, in = e & 7;
+    int at = e;
+    if (!kInter && sub * 8 < a.rot) at = in < 4 ? sub * 4 + in : (a.rot >> 1) + sub * 4 + in - 4;
+    scales[i] = e < a.d ? weight_at(i < kLanes * 8 ? a.r[0].w : a.r[1].w, at, a.w_bf16) : 0.f;
+  }
+}
+__device__ __forceinline__ void fill_table(const Args& a, float2* table, int64_t t0, int nt) {
+  const int half = a.rot >> 1;
+  if (!half) return;
+  const Walk w(threadIdx.x, a.half_inverse, half);  // (an angle per thread: see tile_of)
+  if (w.tk < nt) table[threadIdx.x] = turn_of(a, position_of(a, t0 + w.tk), turns_of(a, w.h));
+}
+
+template <typename T, bool kInter, bool kCache, int kLanes>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4)
+forward_kernel(const Args a) {
+  extern __shared__ __align__(16) float smem[];
+  float2* table = reinterpret_cast<float2*>(smem + 2 * kLanes * 8);
+  rb_pdl_wait();
+  rb_pdl_launch();
+  constexpr int kTurns = sizeof(T) == 2 ? kTurnsBf16 : kTurnsF32, kSize = sizeof(T), kGroups = kThreads / kLanes;
+  using Raw = Raw8<T, kInter>;
+  const Lane l = lane_of<kInter, kLanes>(a);
+  const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
+  const int nt = (int)min((int64_t)a.tokens, a.n - t0);
+  const int hq = a.r[0].heads, hk = a.r[1].heads, rows = hq + hk + (kCache ? hk : 0), half = a.rot >> 1;
+  const bool norm = a.r[0].w != nullptr;
+  const int gap = l.gap * kSize;
+  const char* in_q = reinterpret_cast<const char*>(a.r[0].x) + (t0 * a.r[0].tok + l.at) * kSize;
+  const char* in_k = reinterpret_cast<const char*>(a.r[1].x) + (t0 * a.r[1].tok + l.at) * kSize;
+  const char* in_v = kCache ? reinterpret_cast<const char*>(a.r[2].x) + (t0 * a.r[2].tok + l.at) * kSize : nullptr;
+  char* out_q = reinterpret_cast<char*>(a.r[0].out) + (t0 * hq * a.d + l.at) * kSize;
+  char* out_k = kCache ? nullptr : reinterpret_cast<char*>(a.r[1].out) + (t0 * hk * a.d + l.at) * kSize;
+  const int total = nt * rows, step = gridDim.y * kGroups;
+  Walk fetch(blockIdx.y * kGroups + threadIdx.x / kLanes, a.rows_inverse, rows), use = fetch;
+  bool ready = false;
+  for (int r = blockIdx.y * kGroups; r < total; r += kTurns * step) {
+    Raw raw[kTurns] = {};
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) {
+      if (fetch.tk < nt && l.real) {
+        const bool is_q = fetch.h < hq, is_v = kCache && fetch.h >= hq + hk;
+        const int tok = (int)(is_q ? a.r[0].tok : is_v ? a.r[2].tok : a.r[1].tok), head = (int)(is_q ? a.r[0].head : is_v ? a.r[2].head : a.r[1].head);
+        const int h = is_q ? fetch.h : is_v ? fetch.h - hq - hk : fetch.h - hq;
+        raw[u].load((is_q ? in_q : is_v ? in_v : in_k) + (fetch.tk * tok + h * head) * kSize, gap);
+      }
+      fetch.go(a, rows);
+    }
+    if (!ready) {  // while the first rows are under way
+      fill_scales<kInter, kLanes>(a, smem);
+      fill_table(a, table, t0, nt);
+      __syncthreads();
+      ready = true;
+    }
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) {
+      if (r + u * step < total) {
+        const bool live = use.tk < nt && l.real, is_q = use.h < hq, is_v = kCache && use.h >= hq + hk;
+        F8 y = raw[u].get();
+        if (norm) {
+          const P4 x = pairs(y);
+          const float inv = rsqrtf(group_sum(dot_of(x, x), kLanes) * a.inv_d + a.eps);
+          if (!is_v) y = single(product(scaled(x, inv), scales_at(smem + (is_q ? 0 : kLanes * 8) + l.sub * 8)));
+        }
+        if (live) {
+          if (!is_v) rotate4<kInter>(y, table + use.tk * half, l, 1.f);
+          char* out;
+          if (is_q) {
+            out = out_q + (use.tk * hq + use.h) * (a.d * kSize);
+          } else if (!kCache) {
+            out = out_k + (use.tk * hk + use.h - hq) * (a.d * kSize);
+          } else {
+            const Rows& k = is_v ? a.r[2] : a.r[1];
+            const int64_t at = cache_at(a, k, t0 + use.tk);
+            out = at < 0 ? nullptr : reinterpret_cast<char*>(k.out) + (at + (is_v ? use.h - hq - hk : use.h - hq) * k.page_head + l.at) * kSize;
+          }
+          if (!kCache || out) Raw::store(out, gap, y);
+        }
+        use.go(a, rows);
+      }
     }
   }
 }
 
 // kNorm: x is read again and the weights have gradients (sums per CTA, added up in order by the kernel below)
-template <typename T, bool kInter, bool kNorm>
-__global__ void __launch_bounds__(kThreads)
-backward_kernel(const Args a, int lanes) {
-  extern __shared__ float2 table[];
+template <typename T, bool kInter, bool kNorm, int kLanes>
+__global__ void __launch_bounds__(kThreads, kBackCtas)
+backward_kernel(const Args a) {
+  extern __shared__ __align__(16) float smem[];
+  float2* table = reinterpret_cast<float2*>(smem + 2 * kLanes * 8);
   rb_pdl_wait();
   rb_pdl_launch();
-  const int half = a.rot >> 1;
-  const int sub = threadIdx.x & (lanes - 1);
-  const bool real = sub * 8 < a.d;
-  F8 wq = {}, wk = {}, gq = {}, gk = {};
-  if (kNorm && real) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      wq.v[j] = weight_at(a.wq, sub * 8 + j, a.w_bf16);
-      wk.v[j] = weight_at(a.wk, sub * 8 + j, a.w_bf16);
-    }
-  }
-  const int rows = a.hq + a.hk;
-  const int groups = kThreads / lanes;
-  for (int64_t t0 = (int64_t)blockIdx.x * a.tokens_per_cta; t0 < a.n; t0 += (int64_t)gridDim.x * a.tokens_per_cta) {
-    const int nt = (int)min((int64_t)a.tokens_per_cta, a.n - t0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < nt * half; i += kThreads) table[i] = turn_of(a, t0 + i / half, i % half);
-    __syncthreads();
+  constexpr int kTurns = sizeof(T) == 2 ? kBackBf16 : kBackF32, kSize = sizeof(T), kGroups = kThreads / kLanes;
+  using Raw = Raw8<T, kInter>;
+  const Lane l = lane_of<kInter, kLanes>(a);
+  const int hq = a.r[0].heads, hk = a.r[1].heads, rows = hq + hk, half = a.rot >> 1;
+  const int gap = l.gap * kSize;
+  P4 gq = {}, gk = {};
+  bool have_scales = false;
+  for (int64_t t0 = (int64_t)blockIdx.x * a.tokens; t0 < a.n; t0 += (int64_t)gridDim.x * a.tokens) {
+    const int nt = (int)min((int64_t)a.tokens, a.n - t0);
+    const char* dz_q = reinterpret_cast<const char*>(a.r[0].dz) + (t0 * a.r[0].dz_tok + l.at) * kSize;
+    const char* dz_k = reinterpret_cast<const char*>(a.r[1].dz) + (t0 * a.r[1].dz_tok + l.at) * kSize;
+    const char* in_q = reinterpret_cast<const char*>(a.r[0].x) + (t0 * a.r[0].tok + l.at) * kSize;
+    const char* in_k = reinterpret_cast<const char*>(a.r[1].x) + (t0 * a.r[1].tok + l.at) * kSize;
+    char* out_q = reinterpret_cast<char*>(a.r[0].out) + (t0 * hq * a.d + l.at) * kSize;
+    char* out_k = reinterpret_cast<char*>(a.r[1].out) + (t0 * hk * a.d + l.at) * kSize;
     const int total = nt * rows;
-    for (int r0 = 0; r0 < total; r0 += groups) {
-      const int r = r0 + threadIdx.x / lanes;
-      const bool live = r < total && real;
-      const int tk = live ? r / rows : 0;
-      const int h = live ? r - tk * rows : 0;
-      const int64_t token = t0 + tk;
-      const bool is_q = h < a.hq;
-      F8 g = {}, x = {};
-      if (live) {
-        g = is_q ? load8(a.dq, token * a.dq_tok + h * a.dq_head + sub * 8, is_bf16<T>())
-                 : load8(a.dk, token * a.dk_tok + (h - a.hq) * a.dk_head + sub * 8, is_bf16<T>());
-        if (kNorm) x = is_q ? load8(a.q, token * a.q_tok + h * a.q_head + sub * 8, is_bf16<T>())
-                            : load8(a.k, token * a.k_tok + (h - a.hq) * a.k_head + sub * 8, is_bf16<T>());
-      }
-      rotate8<kInter>(g, table + tk * half, sub, a.rot, -1.f);
-      if (kNorm) {
-        const float inv = rsqrtf(group_sum(squares(x), lanes) / a.d + a.eps);
-        float dot = 0.f;
+    Walk fetch(threadIdx.x / kLanes, a.rows_inverse, rows), use = fetch;
+    for (int r = 0; r < total; r += kTurns * kGroups) {
+      Raw raw_g[kTurns] = {}, raw_x[kNorm ? kTurns : 1] = {};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x.v[j] *= inv;
-          const float c = g.v[j] * x.v[j];  // (zeros in idle lanes)
-          if (is_q) gq.v[j] += c; else gk.v[j] += c;
-          g.v[j] *= is_q ? wq.v[j] : wk.v[j];
-          dot += g.v[j] * x.v[j];
+      for (int u = 0; u < kTurns; ++u) {
+        if (fetch.tk < nt && l.real) {
+          const bool is_q = fetch.h < hq;
+          const int h = is_q ? fetch.h : fetch.h - hq;
+          raw_g[u].load((is_q ? dz_q : dz_k) + (fetch.tk * (int)(is_q ? a.r[0].dz_tok : a.r[1].dz_tok) + h * (int)(is_q ? a.r[0].dz_head : a.r[1].dz_head)) * kSize, gap);
+          if (kNorm) raw_x[u].load((is_q ? in_q : in_k) + (fetch.tk * (int)(is_q ? a.r[0].tok : a.r[1].tok) + h * (int)(is_q ? a.r[0].head : a.r[1].head)) * kSize, gap);
         }
-        dot = group_sum(dot, lanes) / a.d;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g.v[j] = inv * (g.v[j] - x.v[j] * dot);
+        fetch.go(a, rows);
       }
-      if (live) {
-        if (is_q) store8(a.out_q, (token * a.hq + h) * a.d + sub * 8, g, is_bf16<T>());
-        else store8(a.out_k, (token * a.hk + h - a.hq) * a.d + sub * 8, g, is_bf16<T>());
+      if (r == 0) {
+        __syncthreads();  // (the table of the tokens before has been read)
+        if (!have_scales) fill_scales<kInter, kLanes>(a, smem);
+        have_scales = true;
+        fill_table(a, table, t0, nt);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u) {
+        if (r + u * kGroups < total) {
+          const bool live = use.tk < nt && l.real, is_q = use.h < hq;
+          F8 g = raw_g[u].get();
+          if (live) rotate4<kInter>(g, table + use.tk * half, l, -1.f);
+          if (kNorm) {
+            const P4 x = pairs(raw_x[u].get());
+            const float inv = rsqrtf(group_sum(dot_of(x, x), kLanes) * a.inv_d + a.eps);
+            const P4 v = scaled(x, inv), dy = pairs(g);
+            const uint64_t yes = two(is_q ? 1.f : 0.f, is_q ? 1.f : 0.f), no = two(is_q ? 0.f : 1.f, is_q ? 0.f : 1.f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint64_t e = mul2(dy.v[j], v.v[j]);  // (zeros in lanes and groups without a row)
+              gq.v[j] = fma2(e, yes, gq.v[j]);
+              gk.v[j] = fma2(e, no, gk.v[j]);
+            }
+            const P4 w = product(dy, scales_at(smem + (is_q ? 0 : kLanes * 8) + l.sub * 8));
+            const float dot = -group_sum(dot_of(w, v), kLanes) * a.inv_d * inv;
+            const uint64_t by = two(inv, inv), off = two(dot, dot);
+            P4 r;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r.v[j] = fma2(v.v[j], off, mul2(w.v[j], by));
+            g = single(r);
+          }
+          if (live) Raw::store(is_q ? out_q + (use.tk * hq + use.h) * (a.d * kSize) : out_k + (use.tk * hk + use.h - hq) * (a.d * kSize), gap, g);
+          use.go(a, rows);
+        }
       }
     }
   }
   if (kNorm) {
-    float* sums = reinterpret_cast<float*>(table);  // [groups][2][lanes * 8]; at least as large as this (see the launch)
+    float* sums = smem;  // [groups][2][lanes * 8] in the lanes' order; at least as large as this (see the launch)
     __syncthreads();
-    float* mine = sums + (threadIdx.x / lanes) * 2 * lanes * 8;
+    float* mine = sums + threadIdx.x / kLanes * 2 * kLanes * 8;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      mine[sub * 8 + j] = gq.v[j];
-      mine[lanes * 8 + sub * 8 + j] = gk.v[j];
+    for (int j = 0; j < 4; ++j) {
+      reinterpret_cast<uint64_t*>(mine + l.sub * 8)[j] = gq.v[j];
+      reinterpret_cast<uint64_t*>(mine + kLanes * 8 + l.sub * 8)[j] = gk.v[j];
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * a.d; i += kThreads) {
-      const int at = i < a.d ? i : lanes * 8 + i - a.d;
+      const int e = i < a.d ? i : i - a.d, half = a.rot >> 1;
+      int at = e;  // where the lanes have feature e
+      if (!kInter && e < a.rot) at = e < half ? (e >> 2) * 8 + (e & 3) : ((e - half) >> 2) * 8 + 4 + ((e - half) & 3);
+      if (i >= a.d) at += kLanes * 8;
       float s = 0.f;
-      for (int g = 0; g < groups; ++g) s += sums[g * 2 * lanes * 8 + at];
+      for (int g = 0; g < kThreads / kLanes; ++g) s += sums[g * 2 * kLanes * 8 + at];
       a.part[(int64_t)blockIdx.x * 2 * a.d + i] = s;
     }
   }
@@ -267,49 +427,52 @@ template <typename T, bool kCache>
 __global__ void __launch_bounds__(kThreads)
 forward_any_kernel(const Args a) {
   const int lane = threadIdx.x & 31;
-  const int rows = a.hq + a.hk + (kCache ? a.hk : 0);
+  const int rows = a.r[0].heads + a.r[1].heads + (kCache ? a.r[2].heads : 0);
   const int64_t total = a.n * rows;
   rb_pdl_wait();
   rb_pdl_launch();
-  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < total; r += (int64_t)gridDim.x * (kThreads / 32)) {
-    const int64_t token = r / rows;
-    const int h = (int)(r - token * rows);
-    const bool is_q = h < a.hq, value = h >= a.hq + a.hk;
-    const void* x = is_q ? a.q : value ? a.v : a.k;
-    const int64_t base = is_q ? token * a.q_tok + h * a.q_head
-                              : value ? token * a.v_tok + (h - a.hq - a.hk) * a.v_head : token * a.k_tok + (h - a.hq) * a.k_head;
-    const void* w = is_q ? a.wq : a.wk;
+  for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < total; i += (int64_t)gridDim.x * (kThreads / 32)) {
+    const int64_t token = i / rows;
+    int h = (int)(i - token * rows), which = 0;
+    if (h >= a.r[0].heads) {
+      h -= a.r[0].heads;
+      which = 1;
+      if (kCache && h >= a.r[1].heads) {
+        h -= a.r[1].heads;
+        which = 2;
+      }
+    }
+    const Rows& r = a.r[which];
+    const int64_t base = token * r.tok + h * r.head;
     float inv = 1.f;
-    if (w && !value) {
+    if (r.w) {
       float s = 0.f;
       for (int e = lane; e < a.d; e += 32) {
-        const float f = one<T>(x, base + e);
+        const float f = one<T>(r.x, base + e);
         s += f * f;
       }
-      inv = rsqrtf(warp_sum(s) / a.d + a.eps);
+      inv = rsqrtf(warp_sum(s) * a.inv_d + a.eps);
     }
-    void* out = is_q ? a.out_q : kCache ? (value ? a.cache_v : a.cache_k) : a.out_k;
-    int64_t to;
-    if (is_q) to = (token * a.hq + h) * a.d;
-    else if (!kCache) to = (token * a.hk + h - a.hq) * a.d;
-    else if (!value) to = cache_at(a, token, h - a.hq, a.ck_page, a.ck_head, a.ck_tok);
-    else to = cache_at(a, token, h - a.hq - a.hk, a.cv_page, a.cv_head, a.cv_tok);
-    if (to < 0) continue;
+    int64_t to = (token * r.heads + h) * a.d;
+    if (kCache && which) {
+      to = cache_at(a, r, token);
+      if (to < 0) continue;
+      to += h * r.page_head;
+    }
+    const int64_t pos = a.rot && which < 2 ? position_of(a, token) : 0;
     for (int e = lane; e < a.d; e += 32) {
-      float y = one<T>(x, base + e);
-      if (!value) {
-        if (w) y *= inv * weight_at(w, e, a.w_bf16);
-        if (e < a.rot) {
-          int pair;
-          float sign;
-          const int o = partner(e, a.rot, a.interleaved, &pair, &sign);
-          float other = one<T>(x, base + o);
-          if (w) other *= inv * weight_at(w, o, a.w_bf16);
-          const float2 t = turn_of(a, token, pair);
-          y = y * t.x + sign * other * t.y;
-        }
+      float y = one<T>(r.x, base + e);
+      if (r.w) y *= inv * weight_at(r.w, e, a.w_bf16);
+      if (which < 2 && e < a.rot) {
+        int pair;
+        float sign;
+        const int o = partner(e, a.rot, a.interleaved, &pair, &sign);
+        float other = one<T>(r.x, base + o);
+        if (r.w) other *= inv * weight_at(r.w, o, a.w_bf16);
+        const float2 t = turn_of(a, pos, turns_of(a, pair));
+        y = y * t.x + sign * other * t.y;
       }
-      put<T>(out, to + e, y);
+      put<T>(r.out, to + e, y);
     }
   }
 }
@@ -319,58 +482,55 @@ __global__ void __launch_bounds__(kThreads)
 backward_any_kernel(const Args a) {
   __shared__ float sums[kThreads / 32][2][kMaxDim];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rows = a.hq + a.hk;
+  const int rows = a.r[0].heads + a.r[1].heads;
   const int64_t total = a.n * rows;
-  const bool norm = a.wq != nullptr;
+  const bool norm = a.r[0].w != nullptr;
   rb_pdl_wait();
   rb_pdl_launch();
   float gq[kMaxDim / 32] = {}, gk[kMaxDim / 32] = {};
-  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + warp; r < total; r += (int64_t)gridDim.x * (kThreads / 32)) {
-    const int64_t token = r / rows;
-    const int h = (int)(r - token * rows);
-    const bool is_q = h < a.hq;
-    const void* g = is_q ? a.dq : a.dk;
-    const int64_t gb = is_q ? token * a.dq_tok + h * a.dq_head : token * a.dk_tok + (h - a.hq) * a.dk_head;
-    const void* x = is_q ? a.q : a.k;
-    const int64_t xb = is_q ? token * a.q_tok + h * a.q_head : token * a.k_tok + (h - a.hq) * a.k_head;
-    const void* w = is_q ? a.wq : a.wk;
-    void* out = is_q ? a.out_q : a.out_k;
-    const int64_t to = is_q ? (token * a.hq + h) * a.d : (token * a.hk + h - a.hq) * a.d;
+  for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + warp; i < total; i += (int64_t)gridDim.x * (kThreads / 32)) {
+    const int64_t token = i / rows;
+    int h = (int)(i - token * rows);
+    const bool is_q = h < a.r[0].heads;
+    if (!is_q) h -= a.r[0].heads;
+    const Rows& r = a.r[is_q ? 0 : 1];
+    const int64_t gb = token * r.dz_tok + h * r.dz_head, xb = token * r.tok + h * r.head, to = (token * r.heads + h) * a.d;
+    const int64_t pos = a.rot ? position_of(a, token) : 0;
     float inv = 1.f, dot = 0.f;
     float dy[kMaxDim / 32], u[kMaxDim / 32];
     if (norm) {
       float s = 0.f;
       for (int e = lane; e < a.d; e += 32) {
-        const float f = one<T>(x, xb + e);
+        const float f = one<T>(r.x, xb + e);
         s += f * f;
       }
-      inv = rsqrtf(warp_sum(s) / a.d + a.eps);
+      inv = rsqrtf(warp_sum(s) * a.inv_d + a.eps);
     }
 #pragma unroll
     for (int j = 0; j < kMaxDim / 32; ++j) {
       const int e = lane + 32 * j;
       dy[j] = u[j] = 0.f;
       if (e >= a.d) continue;
-      dy[j] = one<T>(g, gb + e);
+      dy[j] = one<T>(r.dz, gb + e);
       if (e < a.rot) {
         int pair;
         float sign;
         const int o = partner(e, a.rot, a.interleaved, &pair, &sign);
-        const float2 t = turn_of(a, token, pair);
-        dy[j] = dy[j] * t.x - sign * one<T>(g, gb + o) * t.y;
+        const float2 t = turn_of(a, pos, turns_of(a, pair));
+        dy[j] = dy[j] * t.x - sign * one<T>(r.dz, gb + o) * t.y;
       }
       if (norm) {
-        u[j] = one<T>(x, xb + e) * inv;
+        u[j] = one<T>(r.x, xb + e) * inv;
         if (is_q) gq[j] += dy[j] * u[j]; else gk[j] += dy[j] * u[j];
-        dy[j] *= weight_at(w, e, a.w_bf16);
+        dy[j] *= weight_at(r.w, e, a.w_bf16);
         dot += dy[j] * u[j];
       }
     }
-    if (norm) dot = warp_sum(dot) / a.d;
+    if (norm) dot = warp_sum(dot) * a.inv_d;
 #pragma unroll
     for (int j = 0; j < kMaxDim / 32; ++j) {
       const int e = lane + 32 * j;
-      if (e < a.d) put<T>(out, to + e, norm ? inv * (dy[j] - u[j] * dot) : dy[j]);
+      if (e < a.d) put<T>(r.out, to + e, norm ? inv * (dy[j] - u[j] * dot) : dy[j]);
     }
   }
   if (norm) {
@@ -415,65 +575,93 @@ weight_sum_kernel(const float* __restrict__ part, int parts, int d, void* __rest
   }
 }
 
+// f of the lanes of a row, 1 to 32, as a constant
+template <typename F>
+auto with_lanes(int d, F f) {
+  if (d <= 8) return f(std::integral_constant<int, 1>());
+  if (d <= 16) return f(std::integral_constant<int, 2>());
+  if (d <= 32) return f(std::integral_constant<int, 4>());
+  if (d <= 64) return f(std::integral_constant<int, 8>());
+  if (d <= 128) return f(std::integral_constant<int, 16>());
+  return f(std::integral_constant<int, 32>());
+}
 int lanes_of(int d) {
-  int l = 1;
-  while (l * 8 < d) l *= 2;
-  return l;
+  return with_lanes(d, [](auto l) { return (int)decltype(l)::value; });
 }
 
-bool aligned(const void* p, std::initializer_list<int64_t> strides, int unit) {
-  if (reinterpret_cast<uintptr_t>(p) & 15) return false;
+bool aligned(const void* p, std::initializer_list<int64_t> strides, int unit, int bytes) {
+  if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
   for (int64_t s : strides)
     if (s % unit) return false;
   return true;
 }
 
-int bad_shape(const Args& a, int backward) {
-  if (a.d < 1 || a.d > kMaxDim || a.rot < 0 || a.rot > a.d || a.rot % 2 || a.hq < 0 || a.hk < 0) {
-    rb_set_error("norm_rope%s: head dim %d (1 to %d), rotated part %d (even, at most the head dim)", backward ? " backward" : "", a.d, kMaxDim, a.rot);
-    return 1;
-  }
-  return 0;
+int bad_shape(const Args& a) {
+  if (a.d >= 1 && a.d <= kMaxDim && a.rot >= 0 && a.rot <= a.d && a.rot % 2 == 0 && a.r[0].heads >= 0 && a.r[1].heads >= 0 && (a.rot == 0 || a.num_pos > 0 || a.n <= 0)) return 0;
+  rb_set_error("norm_rope: head dim %d (1 to %d), rotated part %d (even, at most the head dim)", a.d, kMaxDim, a.rot);
+  return 1;
 }
 
-// 8 features a lane: whole groups of 8, rotated pairs within a lane or a whole number of lanes apart, 16-byte accesses
+// 8 features a lane, whole pairs, vector accesses (16 bytes; pairs (i, i + R / 2) in bf16: 8), tiles below 2^31 bytes
 bool fits(const Args& a, int bf16, bool backward, bool cache) {
-  const int unit = bf16 ? 8 : 4;
-  if (a.d % 8 || (!a.interleaved && a.rot % 16)) return false;
-  bool ok = aligned(a.out_q, {}, unit);
-  if (backward) ok = ok && aligned(a.dq, {a.dq_tok, a.dq_head}, unit) && aligned(a.dk, {a.dk_tok, a.dk_head}, unit) && aligned(a.out_k, {}, unit);
-  if (!backward || a.wq) ok = ok && aligned(a.q, {a.q_tok, a.q_head}, unit) && aligned(a.k, {a.k_tok, a.k_head}, unit);
-  if (cache)
-    ok = ok && aligned(a.v, {a.v_tok, a.v_head}, unit) && aligned(a.cache_k, {a.ck_page, a.ck_head, a.ck_tok}, unit) &&
-         aligned(a.cache_v, {a.cv_page, a.cv_head, a.cv_tok}, unit);
-  else if (!backward) ok = ok && aligned(a.out_k, {}, unit);
+  const int bytes = bf16 && !a.interleaved ? 8 : 16, unit = bytes / (bf16 ? 2 : 4);
+  if (a.d % 8 || a.rot % 8) return false;
+  bool ok = true;
+  for (int i = 0; i < (cache ? 3 : 2); ++i) {
+    const Rows& r = a.r[i];
+    ok = ok && aligned(r.out, {}, unit, bytes);
+    if (!backward || a.r[0].w) ok = ok && aligned(r.x, {r.tok, r.head}, unit, bytes);
+    if (backward) ok = ok && aligned(r.dz, {r.dz_tok, r.dz_head}, unit, bytes);
+    if (cache && i) ok = ok && aligned(r.out, {r.page, r.page_head, r.page_tok}, unit, bytes);
+    // offsets within a tile of up to 256 tokens
+    const int64_t widest = std::max({std::abs(r.head), std::abs(r.dz_head), (int64_t)a.d}) * r.heads + std::max(std::abs(r.tok), std::abs(r.dz_tok)) * 256;
+    ok = ok && widest * 4 < (int64_t)1 << 31 && (int64_t)a.d * r.heads * 256 * 4 < (int64_t)1 << 31;
+  }
   return ok;
 }
 
+// A tile is as many tokens as fill the table with an angle per thread; fewer where that leaves SMs without any
+void tile_of(Args& a) {
+  a.tokens = a.rot ? std::max(1, kThreads / (a.rot / 2)) : 8;
+  while (a.tokens > 1 && (a.n + a.tokens - 1) / a.tokens < 2 * 148) a.tokens /= 2;
+}
+// rows of a tile, `step` groups at a time
+void walk_of(Args& a, int rows, int step) {
+  a.step_tk = step / rows;
+  a.step_h = step % rows;
+  a.rows_inverse = rows > 1 ? (uint32_t)(((1ull << 32) + rows - 1) / rows) : 0u;
+  a.half_inverse = a.rot > 2 ? (uint32_t)(((1ull << 32) + a.rot / 2 - 1) / (a.rot / 2)) : 0u;
+}
+size_t smem_of(const Args& a) { return (size_t)lanes_of(a.d) * 16 * sizeof(float) + (size_t)a.tokens * (a.rot / 2) * sizeof(float2); }
+
+constexpr int kParts = 148 * kBackCtas;
+
 int forward(Args& a, int bf16, bool cache, cudaStream_t stream) {
-  if (bad_shape(a, 0)) return RB_ERR_UNSUPPORTED;
-  const int rows = a.hq + a.hk * (cache ? 2 : 1);
+  if (bad_shape(a)) return RB_ERR_UNSUPPORTED;
+  const int rows = a.r[0].heads + a.r[1].heads * (cache ? 2 : 1);
   if (a.n <= 0 || rows == 0) return RB_OK;
+  a.inv_d = 1.f / a.d;
   if (fits(a, bf16, false, cache)) {
-    const int lanes = lanes_of(a.d), groups = kThreads / lanes, half = a.rot / 2;
-    // a table entry or two per thread, fewer tokens where that leaves SMs without any; then the rows of a token are shared by several CTAs too
-    int tb = half ? max(1, kThreads / half) : 8;
-    while (tb > 1 && (a.n + tb - 1) / tb < 2 * 148) tb /= 2;
-    a.tokens_per_cta = tb;
-    const int64_t gx = (a.n + tb - 1) / tb;
-    int gy = 1;
-    while (gx * gy < 148 && gy * groups * 2 <= tb * rows) gy *= 2;
+    tile_of(a);
+    const int groups = kThreads / lanes_of(a.d);
+    const int64_t gx = (a.n + a.tokens - 1) / a.tokens;
+    int gy = 1;  // where tokens are few their rows are shared by several CTAs
+    while (gx * gy < 148 && gy * groups < a.tokens * rows) gy *= 2;
+    walk_of(a, rows, gy * groups);
     if (gx > 0x7fffffff) {
       rb_set_error("norm_rope: %lld tokens", (long long)a.n);
       return RB_ERR_UNSUPPORTED;
     }
     auto pick = [&](auto t) {
-      using T = decltype(t);
-      return a.interleaved ? (cache ? forward_kernel<T, true, true> : forward_kernel<T, true, false>)
-                           : (cache ? forward_kernel<T, false, true> : forward_kernel<T, false, false>);
+      return with_lanes(a.d, [&](auto l) {
+        using T = decltype(t);
+        constexpr int kL = decltype(l)::value;
+        return a.interleaved ? (cache ? forward_kernel<T, true, true, kL> : forward_kernel<T, true, false, kL>)
+                             : (cache ? forward_kernel<T, false, true, kL> : forward_kernel<T, false, false, kL>);
+      });
     };
     auto kernel = bf16 ? pick(__nv_bfloat16()) : pick(float());
-    rb_launch_pdl(kernel, dim3((unsigned)gx, gy), dim3(kThreads), (size_t)tb * half * sizeof(float2), stream, a, lanes);
+    rb_launch_pdl(kernel, dim3((unsigned)gx, gy), dim3(kThreads), smem_of(a), stream, a);
   } else {
     const int64_t ctas = (a.n * rows + kThreads / 32 - 1) / (kThreads / 32);
     auto kernel = bf16 ? (cache ? forward_any_kernel<__nv_bfloat16, true> : forward_any_kernel<__nv_bfloat16, false>)
@@ -483,15 +671,25 @@ int forward(Args& a, int bf16, bool cache, cudaStream_t stream) {
   return rb_check_launch("norm_rope");
 }
 
+Rows rows_of(const void* x, int64_t tok, int64_t head, int heads, const void* w, void* out) {
+  Rows r = {};
+  r.x = x; r.tok = tok; r.head = head; r.heads = heads; r.w = w; r.out = out;
+  return r;
+}
+void common(Args& a, const void* positions, long long num_pos, const float* freq, long long n, int d, int rot, int pos64, int w_bf16, int interleaved, float eps, float amp) {
+  a.positions = positions; a.num_pos = num_pos; a.freq = freq; a.n = n; a.d = d; a.rot = rot; a.pos64 = pos64; a.w_bf16 = w_bf16; a.interleaved = interleaved;
+  a.eps = eps; a.amp = amp;
+}
+
 }  // namespace
 
 RB_EXPORT int rb200_norm_rope_fwd(const void* q, const void* k, const void* positions, long long num_pos, const float* freq, const void* wq, const void* wk, void* out_q,
                                   void* out_k, const long long* strides /* q token, q head, k token, k head */, long long n, int hq, int hk, int d, int rot,
                                   int bf16, int pos64, int w_bf16, int interleaved, float eps, float amp, cudaStream_t stream) {
   Args a = {};
-  a.q = q; a.k = k; a.positions = positions; a.num_pos = num_pos; a.freq = freq; a.wq = wq; a.wk = wk; a.out_q = out_q; a.out_k = out_k;
-  a.q_tok = strides[0]; a.q_head = strides[1]; a.k_tok = strides[2]; a.k_head = strides[3];
-  a.n = n; a.hq = hq; a.hk = hk; a.d = d; a.rot = rot; a.pos64 = pos64; a.w_bf16 = w_bf16; a.interleaved = interleaved; a.eps = eps; a.amp = amp;
+  a.r[0] = rows_of(q, strides[0], strides[1], hq, wq, out_q);
+  a.r[1] = rows_of(k, strides[2], strides[3], hk, wk, out_k);
+  common(a, positions, num_pos, freq, n, d, rot, pos64, w_bf16, interleaved, eps, amp);
   return forward(a, bf16, false, stream);
 }
 
@@ -505,16 +703,21 @@ RB_EXPORT int rb200_norm_rope_cache(const void* q, const void* k, const void* v,
     rb_set_error("norm_rope: page size %d", page);
     return RB_ERR_ARG;
   }
-  a.q = q; a.k = k; a.v = v; a.positions = positions; a.num_pos = num_pos; a.freq = freq; a.wq = wq; a.wk = wk; a.out_q = out_q;
-  a.cache_k = cache_k; a.cache_v = cache_v; a.slots = slots; a.page = page; a.num_slots = num_slots;
-  a.q_tok = strides[0]; a.q_head = strides[1]; a.k_tok = strides[2]; a.k_head = strides[3]; a.v_tok = strides[4]; a.v_head = strides[5];
-  a.ck_page = strides[6]; a.ck_head = strides[7]; a.ck_tok = strides[8]; a.cv_page = strides[9]; a.cv_head = strides[10]; a.cv_tok = strides[11];
-  a.n = n; a.hq = hq; a.hk = hk; a.d = d; a.rot = rot; a.pos64 = pos64; a.w_bf16 = w_bf16; a.interleaved = interleaved; a.eps = eps; a.amp = amp;
+  a.r[0] = rows_of(q, strides[0], strides[1], hq, wq, out_q);
+  a.r[1] = rows_of(k, strides[2], strides[3], hk, wk, cache_k);
+  a.r[2] = rows_of(v, strides[4], strides[5], hk, nullptr, cache_v);
+  for (int i = 0; i < 2; ++i) {
+    a.r[1 + i].page = strides[6 + 3 * i];
+    a.r[1 + i].page_head = strides[7 + 3 * i];
+    a.r[1 + i].page_tok = strides[8 + 3 * i];
+  }
+  a.slots = slots; a.page = page; a.num_slots = num_slots;
+  common(a, positions, num_pos, freq, n, d, rot, pos64, w_bf16, interleaved, eps, amp);
   return forward(a, bf16, true, stream);
 }
 
 // partial sums that the backward pass leaves: rows of 2 D floats
-RB_EXPORT int rb200_norm_rope_parts() { return 148 * 4; }
+RB_EXPORT int rb200_norm_rope_parts() { return kParts; }
 
 // part: [rb200_norm_rope_parts()][2][D] floats with a norm, else unused; dwq, dwk [D] in the type of the weights
 RB_EXPORT int rb200_norm_rope_bwd(const void* dq, const void* dk, const void* q, const void* k, const void* positions, long long num_pos, const float* freq, const void* wq,
@@ -522,33 +725,35 @@ RB_EXPORT int rb200_norm_rope_bwd(const void* dq, const void* dk, const void* q,
                                   const long long* strides /* dq, dk, q, k: token, head */, long long n, int hq, int hk, int d, int rot, int bf16, int pos64,
                                   int w_bf16, int interleaved, float eps, float amp, cudaStream_t stream) {
   Args a = {};
-  a.dq = dq; a.dk = dk; a.q = q; a.k = k; a.positions = positions; a.num_pos = num_pos; a.freq = freq; a.wq = wq; a.wk = wk; a.out_q = out_q; a.out_k = out_k; a.part = part;
-  a.dq_tok = strides[0]; a.dq_head = strides[1]; a.dk_tok = strides[2]; a.dk_head = strides[3];
-  a.q_tok = strides[4]; a.q_head = strides[5]; a.k_tok = strides[6]; a.k_head = strides[7];
-  a.n = n; a.hq = hq; a.hk = hk; a.d = d; a.rot = rot; a.pos64 = pos64; a.w_bf16 = w_bf16; a.interleaved = interleaved; a.eps = eps; a.amp = amp;
-  if (bad_shape(a, 1)) return RB_ERR_UNSUPPORTED;
+  a.r[0] = rows_of(q, strides[4], strides[5], hq, wq, out_q);
+  a.r[1] = rows_of(k, strides[6], strides[7], hk, wk, out_k);
+  a.r[0].dz = dq; a.r[0].dz_tok = strides[0]; a.r[0].dz_head = strides[1];
+  a.r[1].dz = dk; a.r[1].dz_tok = strides[2]; a.r[1].dz_head = strides[3];
+  a.part = part;
+  common(a, positions, num_pos, freq, n, d, rot, pos64, w_bf16, interleaved, eps, amp);
+  if (bad_shape(a)) return RB_ERR_UNSUPPORTED;
   const bool norm = wq != nullptr;
   const int rows = hq + hk;
   if (!norm && (n <= 0 || rows == 0)) return RB_OK;
+  a.inv_d = 1.f / d;
   int64_t grid;  // (without any row one CTA leaves sums of zero)
   if (fits(a, bf16, true, false)) {
-    const int lanes = lanes_of(d), half = rot / 2;
-    int tb = half ? max(1, kThreads / half) : 8;
-    while (tb > 1 && (n + tb - 1) / tb < 2 * 148) tb /= 2;
-    a.tokens_per_cta = tb;
-    grid = std::max<int64_t>(1, (n + tb - 1) / tb);
-    if (norm) grid = std::min<int64_t>(grid, rb200_norm_rope_parts());
-    grid = std::min<int64_t>(grid, 0x7fffffff);
-    const size_t table = (size_t)tb * half * sizeof(float2), sums = norm ? (size_t)kThreads * 2 * 8 * sizeof(float) : 0;
+    tile_of(a);
+    walk_of(a, std::max(rows, 1), kThreads / lanes_of(d));
+    grid = std::max<int64_t>(1, std::min<int64_t>((n + a.tokens - 1) / a.tokens, kParts));
+    const size_t sums = norm ? (size_t)kThreads * 2 * 8 * sizeof(float) : 0;
     auto pick = [&](auto t) {
-      using T = decltype(t);
-      return interleaved ? (norm ? backward_kernel<T, true, true> : backward_kernel<T, true, false>)
-                         : (norm ? backward_kernel<T, false, true> : backward_kernel<T, false, false>);
+      return with_lanes(d, [&](auto l) {
+        using T = decltype(t);
+        constexpr int kL = decltype(l)::value;
+        return interleaved ? (norm ? backward_kernel<T, true, true, kL> : backward_kernel<T, true, false, kL>)
+                           : (norm ? backward_kernel<T, false, true, kL> : backward_kernel<T, false, false, kL>);
+      });
     };
     auto kernel = bf16 ? pick(__nv_bfloat16()) : pick(float());
-    rb_launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), std::max(table, sums), stream, a, lanes);
+    rb_launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), std::max(smem_of(a), sums), stream, a);
   } else {
-    grid = std::max<int64_t>(1, std::min<int64_t>((n * rows + kThreads / 32 - 1) / (kThreads / 32), rb200_norm_rope_parts()));
+    grid = std::max<int64_t>(1, std::min<int64_t>((n * rows + kThreads / 32 - 1) / (kThreads / 32), kParts));
     auto kernel = bf16 ? backward_any_kernel<__nv_bfloat16> : backward_any_kernel<float>;
     rb_launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
   }

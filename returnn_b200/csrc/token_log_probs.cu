@@ -5,11 +5,14 @@
 // A target outside 0 .. V - 1 has log probability 0 and no gradient of it. A label of logit -inf has probability 0; a row of nothing else has entropy 0,
 // log probabilities -inf and no gradient.
 //
-// Forward: one CTA per row, one pass with a running maximum, sum and sum of exp(z) z; the logits are read once. The K best come without a sort and almost without
-// a second read: the K-th largest of the threads' maxima bounds the K-th largest logit from below, so that only the threads whose maximum reaches the bound
-// look their logits through again (K of 256, each warp one thread's logits at a time), and the few logits above it are ranked by counting.
+// Forward: one CTA per row, one pass with a running maximum, sum and sum of exp(z) z; the logits are read once. A label costs an exponential and, by packed
+// arithmetic, five more instructions; they are what bounds rows of bf16 next to the memory. The K best come without a sort and almost without a second
+// read: the K-th largest of the maxima of 32 groups of threads bounds the K-th largest logit from below, so that only the threads whose maximum reaches the bound
+// look their logits through again, each warp one thread's at a time, and the few logits above it are ranked by counting.
 // Backward: one pass, p from the maximum and the sum; the labels that have a gradient of their own are written once more at the end.
 #include "class_rows.cuh"
+#include "packed_f32.cuh"
+#include <type_traits>
 
 namespace {
 
@@ -17,7 +20,7 @@ using rows::Chunk;
 using rows::ld;
 using rows::row_head;
 
-constexpr int kThreads = 256;
+constexpr int kBack = 256;  // threads of the backward pass
 constexpr int kMaxTop = 32;
 constexpr int kCand = 512;  // logits that are ranked
 constexpr float kLog2e = 1.4426950408889634f;
@@ -53,13 +56,38 @@ struct Stat {
     m = nm;
   }
 };
-// The difference first: the exponent of the maximum is 0 whatever its size, up to the type's lowest value. (One fused multiply-add, x / ln 2 - m / ln 2, would round
-// the second product by 2^-24 of the maximum and overflow at the end of the range.) A logit of -inf has e = 0, which must not meet an infinity.
-__device__ __forceinline__ void add(float x, float m, float& s, float& w, bool entropy) {
+// A logit so far below the maximum that its e is 0: with the entropy, logits are raised to it, so that e = 0 does not meet an infinity. Near the end of
+// the range there is no such number, and the products are guarded one by one.
+__device__ __forceinline__ bool is_far(float m) { return !(fabsf(m) < 1e38f); }
+__device__ __forceinline__ float floor_of(float m) { return m - 1e4f - 0.01f * fabsf(m); }
+// The difference to the maximum first: its exponent is 0 whatever its size, up to the type's lowest value. (One fused multiply-add, x / ln 2 - m / ln 2, would round
+// the second product by 2^-24 of the maximum and overflow at the end of the range.)
+template <bool kEntropy>
+__device__ __forceinline__ void add(float x, float m, float& s, float& w) {
   const float z = x - m;
   const float e = exp2f(z * kLog2e);
   s += e;
-  if (entropy) w += e * fmaxf(z, -1e4f);
+  if (kEntropy) w += e == 0.f ? 0.f : e * z;
+}
+// the logits of a chunk as pairs, raised to `least`
+template <bool kRaise>
+__device__ __forceinline__ void in_pairs(const Chunk<true>& u, float least, uint64_t* p) {
+  const uint32_t w[4] = {u.u.x, u.u.y, u.u.z, u.u.w};
+  const __nv_bfloat162 f = __float2bfloat162_rn(least);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t v = w[i];
+    if (kRaise) {
+      const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), f);
+      v = *reinterpret_cast<const uint32_t*>(&r);
+    }
+    p[i] = two(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+}
+template <bool kRaise>
+__device__ __forceinline__ void in_pairs(const Chunk<false>& u, float least, uint64_t* p) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) p[i] = kRaise ? two(max_nan(u.at(2 * i), least), max_nan(u.at(2 * i + 1), least)) : two(u.at(2 * i), u.at(2 * i + 1));
 }
 
 __device__ __forceinline__ void merge(Stat& a, Stat b) {
@@ -70,21 +98,29 @@ __device__ __forceinline__ void merge(Stat& a, Stat b) {
   a.w += b.w;
 }
 
-// K-th largest of the CTA's 256 whole numbers in shared memory, by one warp, bit by bit (`bits` leading ones may differ)
+// K-th largest of the CTA's whole numbers in shared memory, by one warp, bit by bit (`bits` leading ones may differ)
+template <int kThreads>
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t* key, int k, int bits) {
   const int lane = threadIdx.x & 31;
-  uint32_t mine[kThreads / 32];
-#pragma unroll
-  for (int j = 0; j < kThreads / 32; ++j) mine[j] = key[j * 32 + lane];
   uint32_t found = 0;
   for (int b = 31; b >= 32 - bits; --b) {
     const uint32_t want = found | 1u << b;
     int n = 0;
-#pragma unroll
-    for (int j = 0; j < kThreads / 32; ++j) n += mine[j] >= want;
+    for (int j = 0; j < kThreads / 32; ++j) n += key[j * 32 + lane] >= want;
     if ((int)__reduce_add_sync(0xffffffffu, n) >= k) found = want;
   }
   return found;
+}
+// K-th largest of the 32 whole numbers of a warp
+__device__ __forceinline__ uint32_t kth_of_warp(uint32_t mine, int k) {
+  const int lane = threadIdx.x & 31;
+  int above = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const uint32_t other = __shfl_sync(0xffffffffu, mine, j);
+    above += other > mine || (other == mine && j < lane);
+  }
+  return __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, above == k - 1)) - 1);
 }
 
 struct Row {
@@ -93,18 +129,19 @@ struct Row {
   int head, v8, v;
 };
 
+template <int kThreads>
 struct Best {
-  uint32_t key[kThreads];
+  uint32_t key[kThreads], group[32];
   uint64_t cand[kCand];  // rank of the logit, and the label counted from above
   uint64_t last;
   uint32_t bound, limit;
-  int count, above, equal;
+  int count, above;
 };
 
 __device__ __forceinline__ uint64_t composite(float x, int label) { return (uint64_t)rank_of(x) << 32 | (0xffffffffu - (uint32_t)label); }
 
-template <bool kBf16>
-__device__ __forceinline__ void consider(Best& b, float x, int label) {
+template <int kThreads>
+__device__ __forceinline__ void consider(Best<kThreads>& b, float x, int label) {
   const uint32_t r = rank_of(x);
   if (r > b.bound || (r == b.bound && (uint32_t)label <= b.limit)) {
     const int at = atomicAdd(&b.count, 1);  // (the order does not matter: they are ranked)
@@ -112,31 +149,31 @@ __device__ __forceinline__ void consider(Best& b, float x, int label) {
   }
 }
 
-// logits of the threads whose maximum reaches the bound, and those outside the chunks
-template <bool kBf16>
-__device__ __forceinline__ void collect(Best& b, const Row& r, uint32_t key) {
+// logits of the threads whose maximum reaches the bound, and those outside the chunks; given up where they are too many
+template <int kThreads, bool kBf16>
+__device__ __forceinline__ void collect(Best<kThreads>& b, const Row& r, uint32_t key) {
   constexpr int kN = Chunk<kBf16>::kN;
   const int lane = threadIdx.x & 31;
   uint32_t who = __ballot_sync(0xffffffffu, key >= b.bound);
-  while (who) {
+  while (who && *(volatile int*)&b.count <= kCand) {
     const int t = (threadIdx.x & ~31) + __ffs(who) - 1;
     who &= who - 1;
-    for (int c = r.head + (t + kThreads * lane) * kN; c < r.v8; c += 32 * kThreads * kN) {
+    for (int64_t c = r.head + (t + (int64_t)kThreads * lane) * kN; c < r.v8; c += 32 * kThreads * kN) {
       Chunk<kBf16> u;
       u.load(r.x, r.base + c);
 #pragma unroll
-      for (int k = 0; k < kN; ++k) consider<kBf16>(b, u.at(k), c + k);
+      for (int k = 0; k < kN; ++k) consider(b, u.at(k), (int)c + k);
     }
   }
   const int rest = r.v - (r.v8 - r.head);
   if ((int)threadIdx.x < rest) {
     const int c = (int)threadIdx.x < r.head ? threadIdx.x : threadIdx.x + (r.v8 - r.head);
-    consider<kBf16>(b, ld(r.x, r.base + c, kBf16), c);
+    consider(b, ld(r.x, r.base + c, kBf16), c);
   }
 }
 
 // the first label of this thread's own logits (the chunks, and one outside) that has rank `want`
-template <bool kBf16>
+template <int kThreads, bool kBf16>
 __device__ __forceinline__ uint32_t first_of(const Row& r, uint32_t want) {
   constexpr int kN = Chunk<kBf16>::kN;
   uint32_t at = 0xffffffffu;
@@ -145,93 +182,84 @@ __device__ __forceinline__ uint32_t first_of(const Row& r, uint32_t want) {
     const int c = (int)threadIdx.x < r.head ? threadIdx.x : threadIdx.x + (r.v8 - r.head);
     if (rank_of(ld(r.x, r.base + c, kBf16)) == want) at = c;
   }
-  for (int c = r.head + (int)threadIdx.x * kN; c < r.v8 && (uint32_t)c < at; c += kThreads * kN) {
+  for (int64_t c = r.head + (int)threadIdx.x * kN; c < r.v8 && (uint32_t)c < at; c += kThreads * kN) {
     Chunk<kBf16> u;
     u.load(r.x, r.base + c);
 #pragma unroll
     for (int k = kN - 1; k >= 0; --k)
-      if (rank_of(u.at(k)) == want) at = min(at, (uint32_t)(c + k));
+      if (rank_of(u.at(k)) == want) at = min(at, (uint32_t)c + k);
   }
   return at;
 }
 
-// The K best labels of a row in b.cand, in no order; returns how many there are (at least K; all above the K-th, which is among them).
-// `mx`: the maximum of this thread's chunks and of one logit outside them; `odd`: its sum is no number, the maximum may be one.
-template <bool kBf16>
-__device__ int select(Best& b, const Row& r, int top, float mx, bool odd) {
+// a thread's key: the rank of its largest logit (its chunks, and one outside). `odd`: its sum is no number, the maximum may be one.
+template <int kThreads, bool kBf16>
+__device__ __forceinline__ uint32_t key_of(const Row& r, float mx, bool odd) {
   uint32_t key = rank_of(mx);
   if (odd) {
     constexpr int kN = Chunk<kBf16>::kN;
     const int rest = r.v - (r.v8 - r.head);
     if ((int)threadIdx.x < rest) key = max(key, rank_of(ld(r.x, r.base + ((int)threadIdx.x < r.head ? threadIdx.x : threadIdx.x + (r.v8 - r.head)), kBf16)));
-    for (int c = r.head + (int)threadIdx.x * kN; c < r.v8; c += kThreads * kN)
+    for (int64_t c = r.head + (int)threadIdx.x * kN; c < r.v8; c += kThreads * kN)
       for (int k = 0; k < kN; ++k) key = max(key, rank_of(ld(r.x, r.base + c + k, kBf16)));
   }
+  return key;
+}
+
+// The K best labels of a row in b.cand, in no order; returns how many there are (at least K; all above the K-th, which is among them). b.bound is the K-th largest of the
+// maxima of 32 groups of threads, b.count 0.
+template <int kThreads, bool kBf16>
+__device__ int select(Best<kThreads>& b, const Row& r, int top, uint32_t key) {
+  collect<kThreads, kBf16>(b, r, key);
+  __syncthreads();
+  if (b.count <= kCand) return b.count;
+  // Many equal logits at the bound, or large ones in few groups. With the K-th largest of the threads' own maxima as the bound: of the logits equal to it only those up to the
+  // label that the K best need. The first one of each thread bounds that.
+  __syncthreads();
   b.key[threadIdx.x] = key;
-  if (threadIdx.x == 0) b.count = b.above = b.equal = 0;
+  if (threadIdx.x == 0) b.above = 0;
   __syncthreads();
   if (threadIdx.x < 32) {
     // (the lower half of a bf16 value's rank follows from the upper: zeros, ones where the value is negative or no number)
-    uint32_t bound = kth_largest(b.key, top, kBf16 ? 16 : 32);
+    uint32_t bound = kth_largest<kThreads>(b.key, top, kBf16 ? 16 : 32);
     if (kBf16 && (bound < 0x80000000u || bound == 0xffff0000u)) bound |= 0xffffu;
+    if (threadIdx.x == 0) b.bound = bound;
+  }
+  __syncthreads();
+  const uint32_t bound = b.bound, above = __ballot_sync(0xffffffffu, key > bound);
+  if ((threadIdx.x & 31) == 0 && above) atomicAdd(&b.above, __popc(above));
+  const uint32_t first = key == bound ? first_of<kThreads, kBf16>(r, bound) : 0xffffffffu;
+  b.key[threadIdx.x] = ~first;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const uint32_t limit = ~kth_largest<kThreads>(b.key, top - b.above, 32);
     if (threadIdx.x == 0) {
-      b.bound = bound;
-      b.limit = 0xffffffffu;
+      b.limit = limit;
+      b.count = 0;
     }
   }
   __syncthreads();
-  const unsigned above = __ballot_sync(0xffffffffu, key > b.bound), equal = __ballot_sync(0xffffffffu, key == b.bound);
-  if ((threadIdx.x & 31) == 0) {
-    if (above) atomicAdd(&b.above, __popc(above));
-    if (equal) atomicAdd(&b.equal, __popc(equal));
+  collect<kThreads, kBf16>(b, r, key);
+  __syncthreads();
+  if (b.count <= kCand) return b.count;
+  // more logits above the bound than are ranked (all in few threads' share): the K best one after another
+  uint64_t before = ~0ull;
+  for (int k = 0; k < top; ++k) {
+    uint64_t best = 0;
+    for (int c = threadIdx.x; c < r.v; c += kThreads) {
+      const uint64_t q = composite(ld(r.x, r.base + c, kBf16), c);
+      if (q < before && q > best) best = q;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) b.last = 0;
+    __syncthreads();
+    atomicMax(reinterpret_cast<unsigned long long*>(&b.last), (unsigned long long)best);
+    __syncthreads();
+    before = b.last;
+    if (threadIdx.x == 0) b.cand[k] = before;
   }
   __syncthreads();
-  bool many = b.above + b.equal > 64;
-  if (!many) {
-    collect<kBf16>(b, r, key);
-    __syncthreads();
-    many = b.count > kCand;
-  }
-  if (many) {
-    // many equal logits at the bound: of those, only the ones up to the label that the K best need. A thread's first one bounds it.
-    __syncthreads();
-    const uint32_t bound = b.bound, need = top - b.above;
-    const uint32_t first = key == bound ? first_of<kBf16>(r, bound) : 0xffffffffu;
-    b.key[threadIdx.x] = ~first;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      const uint32_t limit = ~kth_largest(b.key, (int)need, 32);
-      if (threadIdx.x == 0) {
-        b.limit = limit;
-        b.count = 0;
-      }
-    }
-    __syncthreads();
-    collect<kBf16>(b, r, key);
-    __syncthreads();
-    if (b.count > kCand) {
-      // more logits above the bound than are ranked (all in few threads' share): the K best one after another
-      __syncthreads();
-      uint64_t before = ~0ull;
-      for (int k = 0; k < top; ++k) {
-        uint64_t best = 0;
-        for (int c = threadIdx.x; c < r.v; c += kThreads) {
-          const uint64_t q = composite(ld(r.x, r.base + c, kBf16), c);
-          if (q < before && q > best) best = q;
-        }
-        if (threadIdx.x == 0) b.last = 0;
-        __syncthreads();
-        atomicMax(reinterpret_cast<unsigned long long*>(&b.last), (unsigned long long)best);
-        __syncthreads();
-        before = b.last;
-        __syncthreads();
-        if (threadIdx.x == 0) b.cand[k] = before;
-      }
-      if (threadIdx.x == 0) b.count = top;
-      __syncthreads();
-    }
-  }
-  return b.count;
+  return top;
 }
 
 __device__ __forceinline__ float value_of(uint64_t c) {
@@ -244,14 +272,15 @@ __device__ __forceinline__ float log_prob(float x, float2 norm) {
 }
 
 // kBatch: chunks of 16 bytes that a thread has in flight
-template <bool kBf16, bool kEntropy, bool kTop, int kBatch>
+template <int kThreads, bool kBf16, bool kEntropy, bool kTop, int kBatch>
 __global__ void __launch_bounds__(kThreads)
 forward_kernel(const Args a) {
-  constexpr int kN = Chunk<kBf16>::kN;
-  __shared__ float sh_m[8], sh_s[8], sh_w[8];
+  constexpr int kN = Chunk<kBf16>::kN, kWarps = kThreads / 32;
+  __shared__ float sh_m[kWarps], sh_s[kWarps], sh_w[kWarps];
   __shared__ float2 sh_norm;
-  __shared__ Best best;
+  __shared__ Best<kTop ? kThreads : 32> best;
   const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   rb_pdl_wait();
   rb_pdl_launch();
   Row r;
@@ -260,12 +289,22 @@ forward_kernel(const Args a) {
   r.v = a.v;
   r.head = row_head(a.x, r.base, a.v, kBf16 ? 2 : 4);
   r.v8 = r.head + ((a.v - r.head) & ~7);
+  // asked for early, used late: the target's logit (by the thread that finishes the sums), the logits outside the chunks
+  constexpr int kLast = 32;  // of the second warp; the first one looks for the bound
+  long long y = -1;
+  float xy = 0.f, xr = 0.f;
+  if (threadIdx.x == kLast && a.target) {
+    y = target_of(a, row);
+    if (y >= 0 && y < a.v) xy = ld(a.x, r.base + y, kBf16);
+  }
+  const int rest = a.v - (r.v8 - r.head);  // fewer than the threads
+  if ((int)threadIdx.x < rest) xr = ld(a.x, r.base + ((int)threadIdx.x < r.head ? threadIdx.x : threadIdx.x + (r.v8 - r.head)), kBf16);
   Stat st{-INFINITY, 0.f, 0.f};
-  for (int c0 = r.head + threadIdx.x * kN; c0 < r.v8; c0 += kBatch * kThreads * kN) {
+  for (int64_t c0 = r.head + (int)threadIdx.x * kN; c0 < r.v8; c0 += kBatch * kThreads * kN) {
     Chunk<kBf16> u[kBatch];
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) {
-      const int c = c0 + q * kThreads * kN;
+      const int64_t c = c0 + q * kThreads * kN;
       if (c < r.v8) u[q].load(a.x, r.base + c);
       else u[q].fill_neg_inf();
     }
@@ -274,50 +313,95 @@ forward_kernel(const Args a) {
     for (int q = 1; q < kBatch; ++q) lm = fmaxf(lm, u[q].max());
     if (lm > st.m) st.to(lm);
     const float m = st.m == -INFINITY ? 0.f : st.m;
-    float s = 0.f, w = 0.f;
+    if (!is_far(m)) {
+      const float least = kEntropy ? floor_of(m) : 0.f;
+      const uint64_t minus = two(-m, -m), l2 = two(kLog2e, kLog2e);
+      uint64_t s = 0, w = 0;
 #pragma unroll
-    for (int q = 0; q < kBatch; ++q)
-      if (q == 0 || c0 + q * kThreads * kN < r.v8)
+      for (int q = 0; q < kBatch; ++q) {
+        if (q == 0 || c0 + q * kThreads * kN < r.v8) {
+          uint64_t p[kN / 2];
+          in_pairs<kEntropy>(u[q], least, p);
 #pragma unroll
-        for (int k = 0; k < kN; ++k) add(u[q].at(k), m, s, w, kEntropy);
-    st.s += s;
-    st.w += w;
+          for (int k = 0; k < kN / 2; ++k) {
+            const uint64_t z = add2(p[k], minus);
+            float t0, t1;
+            split(mul2(z, l2), t0, t1);
+            const uint64_t e = two(exp2f(t0), exp2f(t1));
+            s = add2(s, e);
+            if (kEntropy) w = fma2(e, z, w);
+          }
+        }
+      }
+      float s0, s1;
+      split(s, s0, s1);
+      st.s += s0 + s1;
+      if (kEntropy) {
+        split(w, s0, s1);
+        st.w += s0 + s1;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q)
+        if (q == 0 || c0 + q * kThreads * kN < r.v8)
+          for (int k = 0; k < kN; ++k) add<kEntropy>(u[q].at(k), m, st.s, st.w);
+    }
   }
-  const int rest = a.v - (r.v8 - r.head);  // fewer than the threads
   if ((int)threadIdx.x < rest) {
-    const int c = (int)threadIdx.x < r.head ? threadIdx.x : threadIdx.x + (r.v8 - r.head);
-    const float x = ld(a.x, r.base + c, kBf16);
-    if (x > st.m) st.to(x);
-    add(x, st.m == -INFINITY ? 0.f : st.m, st.s, st.w, kEntropy);
+    if (xr > st.m) st.to(xr);
+    add<kEntropy>(xr, st.m == -INFINITY ? 0.f : st.m, st.s, st.w);
   }
-  const float mine = st.m;
-  const bool odd = st.s != st.s;
+  uint32_t key = 0;
+  if constexpr (kTop) {
+    key = key_of<kThreads, kBf16>(r, st.m, st.s != st.s);
+    uint32_t g = key;  // of this thread's group: a warp, or 8 lanes of it
+    if (kThreads == 1024) {
+      g = __reduce_max_sync(0xffffffffu, g);
+      if (lane == 0) best.group[warp] = g;
+    } else {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    merge(st, Stat{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.w, o)});
-  const int warp = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) {
+      for (int o = 1; o < 8; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+      if ((lane & 7) == 0) best.group[warp * 4 + (lane >> 3)] = g;
+    }
+  }
+  {
+    const float m = warp_max(st.m);
+    if (m > st.m) st.to(m);
+    st.m = m;
+    st.s = warp_sum(st.s);
+    if (kEntropy) st.w = warp_sum(st.w);
+  }
+  if (lane == 0) {
     sh_m[warp] = st.m;
     sh_s[warp] = st.s;
     sh_w[warp] = st.w;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    st = Stat{sh_m[0], sh_s[0], sh_w[0]};
-#pragma unroll
-    for (int w = 1; w < 8; ++w) merge(st, Stat{sh_m[w], sh_s[w], sh_w[w]});
-    const bool none = st.s == 0.f;  // no label has a probability
-    const float log_s = (float)log((double)st.s);
-    sh_norm = none ? make_float2(0.f, -INFINITY) : make_float2(st.m, log_s);
-    if (a.norm) *reinterpret_cast<float2*>(a.norm + 2 * row) = sh_norm;
-    if (kEntropy) a.entropy[row] = none ? 0.f : log_s - st.w / st.s;
-    if (a.target) {
-      const long long y = target_of(a, row);
-      a.lp[row] = y >= 0 && y < a.v ? log_prob(ld(a.x, r.base + y, kBf16), sh_norm) : 0.f;
+  if constexpr (kTop) {
+    if (warp == 0) {
+    const uint32_t bound = kth_of_warp(best.group[lane], a.top);
+    if (lane == 0) {
+      best.bound = bound;
+      best.limit = 0xffffffffu;
+      best.count = 0;
+    }
     }
   }
-  if (kTop) {
-    const int n = select<kBf16>(best, r, a.top, mine, odd);
+  if (threadIdx.x == kLast) {
+    st = Stat{sh_m[0], sh_s[0], sh_w[0]};
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) merge(st, Stat{sh_m[w], sh_s[w], sh_w[w]});
+    const bool none = st.s == 0.f;  // no label has a probability
+    const float log_s = (float)log((double)st.s);
+    const float2 norm = none ? make_float2(0.f, -INFINITY) : make_float2(st.m, log_s);
+    sh_norm = norm;
+    if (a.norm) *reinterpret_cast<float2*>(a.norm + 2 * row) = norm;
+    if (kEntropy) a.entropy[row] = none ? 0.f : log_s - st.w / st.s;
+    if (a.target) a.lp[row] = y >= 0 && y < a.v ? log_prob(xy, norm) : 0.f;
+  }
+  if constexpr (kTop) {
+    __syncthreads();
+    const int n = select<kThreads, kBf16>(best, r, a.top, key);
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const uint64_t c = best.cand[i];
       int above = 0;
@@ -341,38 +425,35 @@ struct BackArgs {
   int target64, v, top;
 };
 
-template <bool kBf16, bool kEntropy>
-__global__ void __launch_bounds__(kThreads)
+// kTop: the best labels have gradients too. kLastFirst: rows from the last one on.
+template <bool kBf16, bool kEntropy, bool kTop, bool kLastFirst>
+__global__ void __launch_bounds__(kBack)
 backward_kernel(const BackArgs a) {
   __shared__ int label[kMaxTop + 1];
   __shared__ float grad[kMaxTop + 1];
-  const int64_t row = blockIdx.x;
+  const int64_t row = kLastFirst ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
   rb_pdl_wait();
   rb_pdl_launch();
   const int64_t base = row * a.pitch, out = row * (int64_t)a.v;
   const float2 norm = *reinterpret_cast<const float2*>(a.norm + 2 * row);
   const bool none = norm.y == -INFINITY;
-  const int n = a.top + 1;
-  if ((int)threadIdx.x < n) {
-    const int k = threadIdx.x - 1;
-    long long y = -1;
-    float g = 0.f;
-    if (k < 0) {
-      if (a.target && a.d_lp) {
-        y = a.target64 ? reinterpret_cast<const long long*>(a.target)[row] : reinterpret_cast<const int*>(a.target)[row];
-        g = a.d_lp[row * a.d_lp_step];
-      }
-    } else if (a.d_top) {
-      y = a.top_label[row * a.top + k];
-      g = a.d_top[row * a.d_top_row + k * a.d_top_step];
-    }
-    const bool real = !none && y >= 0 && y < a.v;
-    label[threadIdx.x] = real ? (int)y : -1;
-    grad[threadIdx.x] = real ? g : 0.f;
+  long long y = -1;
+  float all = 0.f;  // sum of the gradients of log probabilities
+  if (a.target && a.d_lp) {
+    y = a.target64 ? reinterpret_cast<const long long*>(a.target)[row] : reinterpret_cast<const int*>(a.target)[row];
+    if (none || y < 0 || y >= a.v) y = -1;
+    else all = a.d_lp[row * a.d_lp_step];
   }
-  __syncthreads();
-  float all = 0.f;
-  for (int i = 0; i < n; ++i) all += grad[i];
+  const float own = all;
+  if (kTop) {
+    if ((int)threadIdx.x <= a.top) {
+      const int k = threadIdx.x - 1;
+      label[threadIdx.x] = k < 0 ? (int)y : none ? -1 : a.top_label[row * a.top + k];
+      grad[threadIdx.x] = k < 0 ? own : none ? 0.f : a.d_top[row * a.d_top_row + k * a.d_top_step];
+    }
+    __syncthreads();
+    for (int i = 1; i <= a.top; ++i) all += grad[i];
+  }
   const float ge = kEntropy && !none ? a.d_entropy[row * a.d_entropy_step] : 0.f;
   const float h = kEntropy ? a.entropy[row] : 0.f;
   auto of = [&](float x) {
@@ -383,32 +464,65 @@ backward_kernel(const BackArgs a) {
   const int head_in = row_head(a.x, base, a.v, kBf16 ? 2 : 4), head_out = row_head(a.dx, out, a.v, kBf16 ? 2 : 4);
   const int head = head_in == head_out ? head_in : a.v;  // (rows that are aligned differently: single elements)
   const int v8 = head + ((a.v - head) & ~7);
-#pragma unroll 4
-  for (int c = head + threadIdx.x * 8; c < v8; c += kThreads * 8) {
-    F8 x = load8(a.x, base + c, kBf16);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x.v[k] = of(x.v[k]);
-    store8(a.dx, out + c, x, kBf16);
-  }
-  auto put = [&](int c, float d) {
+  auto put = [&](int64_t c, float d) {
     if (kBf16) reinterpret_cast<__nv_bfloat16*>(a.dx)[out + c] = __float2bfloat16(d);
     else reinterpret_cast<float*>(a.dx)[out + c] = d;
   };
-  for (int i = threadIdx.x; i < a.v - (v8 - head); i += kThreads) {
+  if (!none && !is_far(norm.x)) {
+    const float least = floor_of(norm.x);
+    const uint64_t minus_m = two(-norm.x, -norm.x), minus_s = two(-norm.y, -norm.y), l2 = two(kLog2e, kLog2e), slope = two(-ge, -ge);
+    const float at0 = -(all + ge * h);
+    const uint64_t offset = two(at0, at0);
+#pragma unroll 4
+    for (int64_t c = head + (int)threadIdx.x * 8; c < v8; c += kBack * 8) {
+      constexpr int kN = Chunk<kBf16>::kN;
+      Chunk<kBf16> u[8 / kN];
+#pragma unroll
+      for (int i = 0; i < 8 / kN; ++i) u[i].load(a.x, base + c + i * kN);
+      F8 d;
+#pragma unroll
+      for (int i = 0; i < 8 / kN; ++i) {
+        uint64_t p[kN / 2];
+        in_pairs<kEntropy>(u[i], least, p);
+#pragma unroll
+        for (int k = 0; k < kN / 2; ++k) {
+          const uint64_t lp = add2(add2(p[k], minus_m), minus_s);
+          float t0, t1;
+          split(mul2(lp, l2), t0, t1);
+          const uint64_t e = two(exp2f(t0), exp2f(t1));
+          split(mul2(e, kEntropy ? fma2(lp, slope, offset) : offset), d.v[i * kN + 2 * k], d.v[i * kN + 2 * k + 1]);
+        }
+      }
+      store8(a.dx, out + c, d, kBf16);
+    }
+  } else {
+    for (int64_t c = head + (int)threadIdx.x * 8; c < v8; c += kBack * 8)
+      for (int k = 0; k < 8; ++k) put(c + k, of(ld(a.x, base + c + k, kBf16)));
+  }
+  for (int i = threadIdx.x; i < a.v - (v8 - head); i += kBack) {
     const int c = i < head ? i : i + (v8 - head);
     put(c, of(ld(a.x, base + c, kBf16)));
   }
-  __syncthreads();
-  if ((int)threadIdx.x < n && label[threadIdx.x] >= 0) {
-    const int c = label[threadIdx.x];
-    float own = 0.f;
-    bool first = true;
-    for (int i = 0; i < n; ++i) {
-      if (label[i] != c) continue;
-      if (i < (int)threadIdx.x) first = false;
-      own += grad[i];
+  if (!kTop) {
+    // the target's entry again, by the thread that wrote it
+    if (y >= 0) {
+      const int c = (int)y;
+      const int who = c >= head && c < v8 ? (c - head) / 8 % kBack : (c < head ? c : c - (v8 - head)) % kBack;
+      if ((int)threadIdx.x == who) put(c, own + of(ld(a.x, base + c, kBf16)));
     }
-    if (first) put(c, own + of(ld(a.x, base + c, kBf16)));
+  } else {
+    __syncthreads();
+    if ((int)threadIdx.x <= a.top && label[threadIdx.x] >= 0) {
+      const int c = label[threadIdx.x];
+      float sum = 0.f;
+      bool first = true;
+      for (int i = 0; i <= a.top; ++i) {
+        if (label[i] != c) continue;
+        if (i < (int)threadIdx.x) first = false;
+        sum += grad[i];
+      }
+      if (first) put(c, sum + of(ld(a.x, base + c, kBf16)));
+    }
   }
 }
 
@@ -425,11 +539,20 @@ RB_EXPORT int rb200_token_log_probs_fwd(const void* x, long long pitch, const vo
   Args a = {};
   a.x = x; a.pitch = pitch; a.target = target; a.target64 = target64; a.v = v; a.top = top; a.lp = lp; a.norm = norm; a.entropy = entropy; a.top_lp = top_lp;
   a.top_label = top_label;
-  auto kernel = bf16 ? (entropy ? (top ? forward_kernel<true, true, true, 4> : forward_kernel<true, true, false, 4>)
-                                : (top ? forward_kernel<true, false, true, 4> : forward_kernel<true, false, false, 4>))
-                     : (entropy ? (top ? forward_kernel<false, true, true, 4> : forward_kernel<false, true, false, 4>)
-                                : (top ? forward_kernel<false, false, true, 4> : forward_kernel<false, false, false, 4>));
-  rb_launch_pdl(kernel, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
+  // few rows leave most of the threads to a row of many labels
+  const bool wide = rows <= 2 * 148 && v >= 8192;
+  auto pick = [&](auto threads, auto b) {
+    constexpr int kT = decltype(threads)::value;
+    constexpr bool kB = decltype(b)::value;
+    return entropy ? (top ? forward_kernel<kT, kB, true, true, 4> : forward_kernel<kT, kB, true, false, 4>)
+                   : (top ? forward_kernel<kT, kB, false, true, 4> : forward_kernel<kT, kB, false, false, 4>);
+  };
+  using Few = std::integral_constant<int, 256>;
+  using Many = std::integral_constant<int, 1024>;
+  const std::true_type yes;
+  const std::false_type no;
+  auto kernel = bf16 ? (wide ? pick(Many(), yes) : pick(Few(), yes)) : (wide ? pick(Many(), no) : pick(Few(), no));
+  rb_launch_pdl(kernel, dim3((unsigned)rows), dim3(wide ? 1024 : 256), 0, stream, a);
   return rb_check_launch("token_log_probs_fwd");
 }
 
@@ -444,8 +567,16 @@ RB_EXPORT int rb200_token_log_probs_bwd(const void* x, long long pitch, const vo
   a.x = x; a.pitch = pitch; a.target = target; a.target64 = target64; a.norm = norm; a.entropy = entropy; a.top_label = top_label; a.d_lp = d_lp;
   a.d_lp_step = d_lp_step; a.d_entropy = d_entropy; a.d_entropy_step = d_entropy_step; a.d_top = d_top; a.d_top_row = d_top_row; a.d_top_step = d_top_step;
   a.dx = dx; a.v = v; a.top = d_top ? top : 0;
-  auto kernel = bf16 ? (d_entropy ? backward_kernel<true, true> : backward_kernel<true, false>)
-                     : (d_entropy ? backward_kernel<false, true> : backward_kernel<false, false>);
-  rb_launch_pdl(kernel, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
+  // the last rows first where logits and gradient do not fit the L2 together: what the forward pass read last is what it still holds
+  const bool last_first = rows > 8 * 148 && rows * v * (bf16 ? 2 : 4) >= (64LL << 20);
+  auto pick = [&](auto b) {
+    constexpr bool kB = decltype(b)::value;
+    return d_entropy ? (a.top ? (last_first ? backward_kernel<kB, true, true, true> : backward_kernel<kB, true, true, false>)
+                              : (last_first ? backward_kernel<kB, true, false, true> : backward_kernel<kB, true, false, false>))
+                     : (a.top ? (last_first ? backward_kernel<kB, false, true, true> : backward_kernel<kB, false, true, false>)
+                              : (last_first ? backward_kernel<kB, false, false, true> : backward_kernel<kB, false, false, false>));
+  };
+  auto kernel = bf16 ? pick(std::true_type()) : pick(std::false_type());
+  rb_launch_pdl(kernel, dim3((unsigned)rows), dim3(kBack), 0, stream, a);
   return rb_check_launch("token_log_probs_bwd");
 }
