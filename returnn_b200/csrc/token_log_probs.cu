@@ -23,6 +23,9 @@ using rows::row_head;
 constexpr int kBack = 256;  // threads of the backward pass
 constexpr int kMaxTop = 32;
 constexpr int kCand = 512;  // logits that are ranked
+// Up to this many best the bound comes from 32 groups of threads (32 shuffles; 12 of 32 are reached by 15 logits on the average), beyond from the threads themselves (a search bit by
+// bit, about a microsecond; 32 of 32 groups would be reached by 130). 1500 rows x 10001 fp32, 32 best: 60 and 31 us
+constexpr int kFewTop = 12;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -134,18 +137,20 @@ struct Best {
   uint32_t key[kThreads], group[32];
   uint64_t cand[kCand];  // rank of the logit, and the label counted from above
   uint64_t last;
-  uint32_t bound, limit;
-  int count, above;
+  uint32_t bound;
+  int count, found[kThreads / 32];
 };
 
-__device__ __forceinline__ uint64_t composite(float x, int label) { return (uint64_t)rank_of(x) << 32 | (0xffffffffu - (uint32_t)label); }
+// orders logits by rank, then by label from the lowest; below ~0
+__device__ __forceinline__ uint64_t composite(uint32_t rank, int label) { return (uint64_t)rank << 32 | (0xfffffffeu - (uint32_t)label); }
+__device__ __forceinline__ int label_of(uint64_t c) { return (int)(0xfffffffeu - (uint32_t)c); }
 
 template <int kThreads>
 __device__ __forceinline__ void consider(Best<kThreads>& b, float x, int label) {
   const uint32_t r = rank_of(x);
-  if (r > b.bound || (r == b.bound && (uint32_t)label <= b.limit)) {
+  if (r >= b.bound) {
     const int at = atomicAdd(&b.count, 1);  // (the order does not matter: they are ranked)
-    if (at < kCand) b.cand[at] = (uint64_t)r << 32 | (0xffffffffu - (uint32_t)label);
+    if (at < kCand) b.cand[at] = composite(r, label);
   }
 }
 
@@ -156,11 +161,13 @@ __device__ __forceinline__ void collect(Best<kThreads>& b, const Row& r, uint32_
   const int lane = threadIdx.x & 31;
   uint32_t who = __ballot_sync(0xffffffffu, key >= b.bound);
   while (who && *(volatile int*)&b.count <= kCand) {
-    const int t = (threadIdx.x & ~31) + __ffs(who) - 1;
+    const int t = __ffs(who) - 1;
     who &= who - 1;
-    for (int64_t c = r.head + (t + (int64_t)kThreads * lane) * kN; c < r.v8; c += 32 * kThreads * kN) {
+    const bool odd = __shfl_sync(0xffffffffu, key, t) == 0xffffffffu;  // (a maximum passes a NaN by)
+    for (int64_t c = r.head + ((threadIdx.x & ~31) + t + (int64_t)kThreads * lane) * kN; c < r.v8; c += 32 * kThreads * kN) {
       Chunk<kBf16> u;
       u.load(r.x, r.base + c);
+      if (!odd && rank_of(u.max()) < b.bound) continue;
 #pragma unroll
       for (int k = 0; k < kN; ++k) consider(b, u.at(k), (int)c + k);
     }
@@ -170,26 +177,6 @@ __device__ __forceinline__ void collect(Best<kThreads>& b, const Row& r, uint32_
     const int c = (int)threadIdx.x < r.head ? threadIdx.x : threadIdx.x + (r.v8 - r.head);
     consider(b, ld(r.x, r.base + c, kBf16), c);
   }
-}
-
-// the first label of this thread's own logits (the chunks, and one outside) that has rank `want`
-template <int kThreads, bool kBf16>
-__device__ __forceinline__ uint32_t first_of(const Row& r, uint32_t want) {
-  constexpr int kN = Chunk<kBf16>::kN;
-  uint32_t at = 0xffffffffu;
-  const int rest = r.v - (r.v8 - r.head);
-  if ((int)threadIdx.x < rest) {
-    const int c = (int)threadIdx.x < r.head ? threadIdx.x : threadIdx.x + (r.v8 - r.head);
-    if (rank_of(ld(r.x, r.base + c, kBf16)) == want) at = c;
-  }
-  for (int64_t c = r.head + (int)threadIdx.x * kN; c < r.v8 && (uint32_t)c < at; c += kThreads * kN) {
-    Chunk<kBf16> u;
-    u.load(r.x, r.base + c);
-#pragma unroll
-    for (int k = kN - 1; k >= 0; --k)
-      if (rank_of(u.at(k)) == want) at = min(at, (uint32_t)c + k);
-  }
-  return at;
 }
 
 // a thread's key: the rank of its largest logit (its chunks, and one outside). `odd`: its sum is no number, the maximum may be one.
@@ -206,48 +193,65 @@ __device__ __forceinline__ uint32_t key_of(const Row& r, float mx, bool odd) {
   return key;
 }
 
-// The K best labels of a row in b.cand, in no order; returns how many there are (at least K; all above the K-th, which is among them). b.bound is the K-th largest of the
-// maxima of 32 groups of threads, b.count 0.
+// K-th largest of the threads' keys, by the first warp
+template <int kThreads, bool kBf16>
+__device__ __forceinline__ uint32_t bound_of_threads(const Best<kThreads>& b, int top) {
+  // (the lower half of a bf16 value's rank follows from the upper: zeros, ones where the value is negative or no number)
+  uint32_t bound = kth_largest<kThreads>(b.key, top, kBf16 ? 16 : 32);
+  if (kBf16 && (bound < 0x80000000u || bound == 0xffff0000u)) bound |= 0xffffu;
+  return bound;
+}
+
+// The K best labels of a row in b.cand, in no order; returns how many there are (at least K, all above the K-th and itself among them). b.bound: at most the rank of the
+// K-th largest logit; b.count: 0
 template <int kThreads, bool kBf16>
 __device__ int select(Best<kThreads>& b, const Row& r, int top, uint32_t key) {
   collect<kThreads, kBf16>(b, r, key);
   __syncthreads();
   if (b.count <= kCand) return b.count;
-  // Many equal logits at the bound, or large ones in few groups. With the K-th largest of the threads' own maxima as the bound: of the logits equal to it only those up to the
-  // label that the K best need. The first one of each thread bounds that.
+  // Many equal logits at the bound (masks), or large ones in few groups. With the K-th largest of the threads' maxima as the bound, the logits above it lie in fewer than K
+  // threads; of those equal to it the lowest labels are taken, in order, a stretch of labels after another.
   __syncthreads();
   b.key[threadIdx.x] = key;
-  if (threadIdx.x == 0) b.above = 0;
+  if (threadIdx.x == 0) b.count = 0;
   __syncthreads();
   if (threadIdx.x < 32) {
-    // (the lower half of a bf16 value's rank follows from the upper: zeros, ones where the value is negative or no number)
-    uint32_t bound = kth_largest<kThreads>(b.key, top, kBf16 ? 16 : 32);
-    if (kBf16 && (bound < 0x80000000u || bound == 0xffff0000u)) bound |= 0xffffu;
+    const uint32_t bound = bound_of_threads<kThreads, kBf16>(b, top);
     if (threadIdx.x == 0) b.bound = bound;
   }
   __syncthreads();
-  const uint32_t bound = b.bound, above = __ballot_sync(0xffffffffu, key > bound);
-  if ((threadIdx.x & 31) == 0 && above) atomicAdd(&b.above, __popc(above));
-  const uint32_t first = key == bound ? first_of<kThreads, kBf16>(r, bound) : 0xffffffffu;
-  b.key[threadIdx.x] = ~first;
+  const uint32_t bound = b.bound;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const uint32_t limit = ~kth_largest<kThreads>(b.key, top - b.above, 32);
-    if (threadIdx.x == 0) {
-      b.limit = limit;
-      b.count = 0;
+  if (threadIdx.x == 0) b.bound = bound + 1;
+  __syncthreads();
+  if (bound != 0xffffffffu) collect<kThreads, kBf16>(b, r, key);  // (nothing is above a NaN)
+  __syncthreads();
+  int have = b.count;
+  if (have <= kCand) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int c0 = 0; c0 < r.v && have < top; c0 += kThreads) {
+      const int c = c0 + threadIdx.x;
+      const uint32_t yes = __ballot_sync(0xffffffffu, c < r.v && rank_of(ld(r.x, r.base + c, kBf16)) == bound);
+      if (lane == 0) b.found[warp] = __popc(yes);
+      __syncthreads();
+      int at = have, all = have;
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) at += b.found[w];
+        all += b.found[w];
+      }
+      at += __popc(yes & ((1u << lane) - 1u));
+      if ((yes >> lane & 1) && at < top) b.cand[at] = composite(bound, c);
+      have = all;
+      __syncthreads();
     }
+    return min(have, max(b.count, top));
   }
-  __syncthreads();
-  collect<kThreads, kBf16>(b, r, key);
-  __syncthreads();
-  if (b.count <= kCand) return b.count;
   // more logits above the bound than are ranked (all in few threads' share): the K best one after another
   uint64_t before = ~0ull;
   for (int k = 0; k < top; ++k) {
     uint64_t best = 0;
     for (int c = threadIdx.x; c < r.v; c += kThreads) {
-      const uint64_t q = composite(ld(r.x, r.base + c, kBf16), c);
+      const uint64_t q = composite(rank_of(ld(r.x, r.base + c, kBf16)), c);
       if (q < before && q > best) best = q;
     }
     __syncthreads();
@@ -273,7 +277,7 @@ __device__ __forceinline__ float log_prob(float x, float2 norm) {
 
 // kBatch: chunks of 16 bytes that a thread has in flight
 template <int kThreads, bool kBf16, bool kEntropy, bool kTop, int kBatch>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 6 : 1)
 forward_kernel(const Args a) {
   constexpr int kN = Chunk<kBf16>::kN, kWarps = kThreads / 32;
   __shared__ float sh_m[kWarps], sh_s[kWarps], sh_w[kWarps];
@@ -354,14 +358,18 @@ forward_kernel(const Args a) {
   uint32_t key = 0;
   if constexpr (kTop) {
     key = key_of<kThreads, kBf16>(r, st.m, st.s != st.s);
-    uint32_t g = key;  // of this thread's group: a warp, or 8 lanes of it
-    if (kThreads == 1024) {
-      g = __reduce_max_sync(0xffffffffu, g);
-      if (lane == 0) best.group[warp] = g;
-    } else {
+    if (a.top <= kFewTop) {
+      uint32_t g = key;  // of this thread's group: a warp, or 8 lanes of it
+      if (kThreads == 1024) {
+        g = __reduce_max_sync(0xffffffffu, g);
+        if (lane == 0) best.group[warp] = g;
+      } else {
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-      if ((lane & 7) == 0) best.group[warp * 4 + (lane >> 3)] = g;
+        for (int o = 1; o < 8; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if ((lane & 7) == 0) best.group[warp * 4 + (lane >> 3)] = g;
+      }
+    } else {
+      best.key[threadIdx.x] = key;
     }
   }
   {
@@ -379,10 +387,9 @@ forward_kernel(const Args a) {
   __syncthreads();
   if constexpr (kTop) {
     if (warp == 0) {
-    const uint32_t bound = kth_of_warp(best.group[lane], a.top);
+    const uint32_t bound = a.top <= kFewTop ? kth_of_warp(best.group[lane], a.top) : bound_of_threads<kThreads, kBf16>(best, a.top);
     if (lane == 0) {
       best.bound = bound;
-      best.limit = 0xffffffffu;
       best.count = 0;
     }
     }
@@ -401,13 +408,20 @@ forward_kernel(const Args a) {
   }
   if constexpr (kTop) {
     __syncthreads();
+    if (sh_norm.y == -INFINITY) {  // a row of nothing but -inf
+      if ((int)threadIdx.x < a.top) {
+        a.top_label[row * a.top + threadIdx.x] = threadIdx.x;
+        a.top_lp[row * a.top + threadIdx.x] = -INFINITY;
+      }
+      return;
+    }
     const int n = select<kThreads, kBf16>(best, r, a.top, key);
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const uint64_t c = best.cand[i];
       int above = 0;
       for (int j = 0; j < n; ++j) above += best.cand[j] > c;
       if (above < a.top) {
-        a.top_label[row * a.top + above] = (int)(0xffffffffu - (uint32_t)c);
+        a.top_label[row * a.top + above] = label_of(c);
         a.top_lp[row * a.top + above] = log_prob(value_of(c), sh_norm);
       }
     }
