@@ -92,13 +92,13 @@ def append_tokens(block_table: torch.Tensor, lengths: torch.Tensor, counts: torc
         dev = block_table.device
         n, blocks = block_table.shape
         lengths, counts, free_range = lengths.contiguous(), counts.contiguous(), free_range.contiguous()
-        lists = torch.empty(3, max_tokens, dtype=torch.int32, device=dev)
+        lists = torch.empty(3, (max_tokens + 3) // 4 * 4, dtype=torch.int32, device=dev)
         offsets = torch.empty(n + 1, dtype=torch.int32, device=dev)
         new_lengths = torch.empty(n, dtype=torch.int32, device=dev)
         new_range = torch.empty(2, dtype=torch.int64, device=dev)
         granted = torch.empty(n, dtype=torch.bool, device=dev)
         fn = _lib.bind("rb200_paged_append", [_vp, _i64, _i32, _vp, _vp, _i32, _vp, _i64, _vp, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp])
-        slots, positions, requests = lists.unbind(0)
+        slots, positions, requests = lists[:, :max_tokens].unbind(0)
         _lib.check(fn(block_table.data_ptr(), block_table.stride(0), blocks, lengths.data_ptr(), counts.data_ptr(), n, free_pages.data_ptr(), free_pages.shape[0],
                       free_range.data_ptr(), page_size, max_tokens, slots.data_ptr(), positions.data_ptr(), requests.data_ptr(), offsets.data_ptr(),
                       new_lengths.data_ptr(), new_range.data_ptr(), granted.data_ptr(), _lib.stream_ptr()), what)
