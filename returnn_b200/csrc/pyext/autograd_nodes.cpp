@@ -1,5 +1,5 @@
 // Autograd nodes of operators that a model calls in every layer: layer norm, linear layer, convolution module, attention with head dim 64, softmax
-// cross entropy. They allocate and launch what the Python functions of returnn_b200/ops do (which stay for traced
+// cross entropy, rotary positions, log probabilities of tokens; and, without a gradient, the operators around a paged cache. They allocate and launch what the Python functions of returnn_b200/ops do (which stay for traced
 // programs), without the interpreter: in the backward pass the engine's thread does not wait for the GIL. A layer norm of 6656 x 512, forward and
 // backward, is 16 us of kernels; its calls took 122 us. The kernels are those of librb200.so.
 //
@@ -14,6 +14,9 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <atomic>
+#include <climits>
+#include <initializer_list>
+#include <utility>
 
 using at::Tensor;
 using torch::autograd::AutogradContext;
@@ -51,6 +54,30 @@ int rb200_softmax_ce_fwd(const void* logits, const int* targets, float* loss, fl
                          int* amax, cudaStream_t stream);
 int rb200_softmax_ce_bwd(const void* logits, const int* targets, const float* lse, const float* dloss, void* dlogits, long long rows, int v, float smoothing,
                          int is_bf16, int grad_only, cudaStream_t stream);
+int rb200_norm_rope_fwd(const void* q, const void* k, const void* positions, long long num_pos, const float* freq, const void* wq, const void* wk, void* out_q,
+                        void* out_k, const long long* strides, long long n, int hq, int hk, int d, int rot, int bf16, int pos64, int w_bf16, int interleaved, float eps,
+                        float amp, cudaStream_t stream);
+int rb200_norm_rope_cache(const void* q, const void* k, const void* v, const void* positions, long long num_pos, const float* freq, const void* wq, const void* wk,
+                          void* out_q, void* cache_k, void* cache_v, const int* slots, const long long* strides, long long n, int hq, int hk, int d, int rot, int page,
+                          long long num_slots, int bf16, int pos64, int w_bf16, int interleaved, float eps, float amp, cudaStream_t stream);
+int rb200_norm_rope_parts();
+int rb200_norm_rope_bwd(const void* dq, const void* dk, const void* q, const void* k, const void* positions, long long num_pos, const float* freq, const void* wq,
+                        const void* wk, void* out_q, void* out_k, float* part, void* dwq, void* dwk, const long long* strides, long long n, int hq, int hk, int d, int rot,
+                        int bf16, int pos64, int w_bf16, int interleaved, float eps, float amp, cudaStream_t stream);
+int rb200_paged_append(int* table, long long table_stride, int blocks, const int* lens, const int* add, int n, int* ring, long long ring_size, const long long* range,
+                       int page, long long max_tokens, int* slots, int* positions, int* requests, int* offsets, int* new_lens, long long* new_range, void* granted,
+                       cudaStream_t stream);
+int rb200_paged_release(const int* table, long long table_stride, int blocks, const int* lens, const void* done, int n, int* ring, long long ring_size,
+                        const long long* range, int page, int* new_lens, long long* new_range, cudaStream_t stream);
+long long rb200_paged_attention_workspace(int n, int heads, int kv_heads, int d, int bf16);
+int rb200_paged_attention(const void* q, const void* k, const void* v, const int* table, long long table_stride, const int* lens, void* out, void* workspace,
+                          const long long* strides, int n, int heads, int kv_heads, int d, int page, int blocks, int num_pages, float scale, int bf16, int* status,
+                          cudaStream_t stream);
+int rb200_token_log_probs_fwd(const void* x, long long pitch, const void* target, int target64, long long rows, int v, int top, int bf16, float* lp, float* norm,
+                              float* entropy, float* top_lp, int* top_label, cudaStream_t stream);
+int rb200_token_log_probs_bwd(const void* x, long long pitch, const void* target, int target64, const float* norm, const float* entropy, const int* top_label,
+                              const float* d_lp, long long d_lp_step, const float* d_entropy, long long d_entropy_step, const float* d_top, long long d_top_row,
+                              long long d_top_step, void* dx, long long rows, int v, int top, int bf16, cudaStream_t stream);
 }
 
 namespace {
@@ -440,6 +467,265 @@ struct CrossEntropy : Function<CrossEntropy> {
   }
 };
 
+// ---- operators of a served language model. Arguments that are not the plain case give nothing (the Python functions look closer: they copy, refuse, or run elsewhere).
+bool bf16_or_fp32(const Tensor& t) { return is_bf16(t) || t.scalar_type() == at::kFloat; }
+bool wants_gradient(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (t && t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+struct RopeArgs {
+  Tensor positions, frequencies, wq, wk;  // undefined: none
+  double eps, amp;
+  bool interleaved;
+  int64_t count = 1, rot = 0;
+  bool is64() const { return positions.defined() && positions.scalar_type() == at::kLong; }
+  bool w_bf16() const { return wq.defined() && is_bf16(wq); }
+  bool fits(const Tensor& q, const Tensor& k) {
+    const int64_t n = q.dim(), d = n ? q.size(-1) : 0;
+    if (n < 3 || k.dim() != n || !q.is_cuda() || k.device() != q.device() || !bf16_or_fp32(q) || k.scalar_type() != q.scalar_type() || k.size(-1) != d || d > 256) return false;
+    for (int64_t i = 0; i + 2 < n; ++i)
+      if (q.size(i) != k.size(i)) return false;
+    if (frequencies.defined()) {
+      if (!positions.defined() || (positions.scalar_type() != at::kInt && positions.scalar_type() != at::kLong) || positions.device() != q.device() ||
+          frequencies.device() != q.device() || frequencies.dim() != 1 || frequencies.scalar_type() != at::kFloat || 2 * frequencies.size(0) > d || positions.dim() > n - 2)
+        return false;
+      for (int64_t i = 0; i < positions.dim(); ++i)
+        if (positions.size(i) != q.size(n - 2 - positions.dim() + i)) return false;
+      count = positions.numel();
+      rot = 2 * frequencies.size(0);
+      positions = positions.contiguous();
+      frequencies = frequencies.contiguous();
+    } else {
+      positions = Tensor();
+    }
+    if (wq.defined() != wk.defined()) return false;
+    if (wq.defined()) {
+      for (const Tensor* w : {&wq, &wk})
+        if (w->dim() != 1 || w->size(0) != d || w->scalar_type() != wq.scalar_type() || w->device() != q.device()) return false;
+      if (!bf16_or_fp32(wq)) return false;
+    }
+    return true;
+  }
+};
+// [..., heads, D] -> [N, heads, D] with unit stride over D
+Tensor token_rows(const Tensor& x) {
+  const Tensor y = x.dim() == 3 ? x : x.reshape({-1, x.size(-2), x.size(-1)});
+  return y.stride(2) == 1 || y.size(2) == 1 ? y : y.contiguous();
+}
+void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+std::pair<Tensor, Tensor> norm_rope_forward(const Tensor& q, const Tensor& q3, const Tensor& k, const Tensor& k3, const RopeArgs& a, const Tensor& wq, const Tensor& wk) {
+  Tensor out_q = fresh(q.sizes(), q, q.scalar_type()), out_k = fresh(k.sizes(), q, q.scalar_type());
+  const long long st[4] = {q3.stride(0), q3.stride(1), k3.stride(0), k3.stride(1)};
+  check(rb200_norm_rope_fwd(ptr(q3), ptr(k3), data(a.positions), a.count, (const float*)data(a.frequencies), data(wq), data(wk), ptr(out_q), ptr(out_k), st, q3.size(0),
+                            (int)q3.size(1), (int)k3.size(1), (int)q3.size(2), (int)a.rot, is_bf16(q), a.is64(), a.w_bf16(), a.interleaved, (float)a.eps, (float)a.amp,
+                            stream()),
+        "norm_rope");
+  count();
+  return {out_q, out_k};
+}
+
+struct NormRope : Function<NormRope> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& wq_, const OptTensor& wk_, const RopeArgs& a) {
+    const Tensor q3 = token_rows(q), k3 = token_rows(k), wq = wq_.has_value() ? wq_->contiguous() : Tensor(), wk = wk_.has_value() ? wk_->contiguous() : Tensor();
+    auto [out_q, out_k] = norm_rope_forward(q, q3, k, k3, a, wq, wk);
+    // without a norm the gradient is a rotation back: the inputs are not kept
+    ctx->save_for_backward({wq.defined() ? q3 : Tensor(), wq.defined() ? k3 : Tensor(), a.positions, a.frequencies, wq, wk});
+    auto& d = ctx->saved_data;
+    d["eps"] = a.eps;
+    d["amp"] = a.amp;
+    d["interleaved"] = a.interleaved;
+    d["count"] = a.count;
+    d["rot"] = a.rot;
+    d["q"] = q.sizes().vec();
+    d["k"] = k.sizes().vec();
+    return {out_q, out_k};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &q3 = s[0], &k3 = s[1], &positions = s[2], &frequencies = s[3], &wq = s[4], &wk = s[5];
+    auto& d = ctx->saved_data;
+    const c10::cuda::CUDAGuard guard(grads[0].device());
+    const Tensor dq = token_rows(grads[0]), dk = token_rows(grads[1]);
+    const int64_t dim = dq.size(2);
+    Tensor gq = fresh(d["q"].toIntVector(), dq, dq.scalar_type()), gk = fresh(d["k"].toIntVector(), dq, dq.scalar_type()), part, dwq, dwk;
+    if (wq.defined()) {
+      part = fresh({rb200_norm_rope_parts(), 2 * dim}, dq, at::kFloat);
+      dwq = fresh_like(wq);
+      dwk = fresh_like(wk);
+    }
+    const bool norm = wq.defined();
+    const long long st[8] = {dq.stride(0), dq.stride(1), dk.stride(0), dk.stride(1), norm ? q3.stride(0) : 0, norm ? q3.stride(1) : 0, norm ? k3.stride(0) : 0,
+                             norm ? k3.stride(1) : 0};
+    check(rb200_norm_rope_bwd(ptr(dq), ptr(dk), data(q3), data(k3), data(positions), d["count"].toInt(), (const float*)data(frequencies), data(wq), data(wk), ptr(gq), ptr(gk),
+                              (float*)data(part), data(dwq), data(dwk), st, dq.size(0), (int)dq.size(1), (int)dk.size(1), (int)dim, (int)d["rot"].toInt(), is_bf16(dq),
+                              positions.defined() && positions.scalar_type() == at::kLong, norm && is_bf16(wq), d["interleaved"].toBool(), (float)d["eps"].toDouble(),
+                              (float)d["amp"].toDouble(), stream()),
+          "norm_rope_bwd");
+    count(norm ? 2 : 1);
+    return {gq, gk, dwq, dwk, Tensor()};
+  }
+};
+
+variable_list norm_rope(const Tensor& q, const Tensor& k, RopeArgs a) {
+  if (!a.fits(q, k)) return {};
+  const c10::cuda::CUDAGuard guard(q.device());
+  if (wants_gradient({&q, &k, &a.wq, &a.wk})) return NormRope::apply(q, k, a.wq.defined() ? OptTensor(a.wq) : OptTensor(), a.wk.defined() ? OptTensor(a.wk) : OptTensor(), a);
+  auto [out_q, out_k] = norm_rope_forward(q, token_rows(q), k, token_rows(k), a, a.wq.defined() ? a.wq.contiguous() : a.wq, a.wk.defined() ? a.wk.contiguous() : a.wk);
+  return {out_q, out_k};
+}
+
+Tensor norm_rope_to_cache(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cache_k, const Tensor& cache_v, const Tensor& slots, RopeArgs a) {
+  if (q.dim() != 3 || !a.fits(q, k) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || v.device() != q.device() ||
+      wants_gradient({&q, &k, &v, &a.wq, &a.wk}))
+    return {};
+  for (const Tensor* c : {&cache_k, &cache_v})
+    if (c->dim() != 4 || c->size(1) != k.size(1) || c->size(3) != k.size(2) || c->sizes() != cache_k.sizes() || c->scalar_type() != q.scalar_type() ||
+        c->device() != q.device() || c->stride(3) != 1 || c->size(2) < 1)
+      return {};
+  if (slots.dim() != 1 || slots.size(0) != q.size(0) || slots.scalar_type() != at::kInt || slots.device() != q.device()) return {};
+  const c10::cuda::CUDAGuard guard(q.device());
+  const Tensor q3 = token_rows(q), k3 = token_rows(k), v3 = token_rows(v), at = slots.contiguous(), wq = a.wq.defined() ? a.wq.contiguous() : a.wq,
+               wk = a.wk.defined() ? a.wk.contiguous() : a.wk;
+  Tensor out = fresh(q.sizes(), q, q.scalar_type());
+  const long long st[12] = {q3.stride(0),      q3.stride(1),      k3.stride(0),      k3.stride(1),      v3.stride(0),      v3.stride(1),
+                            cache_k.stride(0), cache_k.stride(1), cache_k.stride(2), cache_v.stride(0), cache_v.stride(1), cache_v.stride(2)};
+  check(rb200_norm_rope_cache(ptr(q3), ptr(k3), ptr(v3), data(a.positions), a.count, (const float*)data(a.frequencies), data(wq), data(wk), ptr(out), ptr(cache_k),
+                              ptr(cache_v), ptr<int>(at), st, q3.size(0), (int)q3.size(1), (int)k3.size(1), (int)q3.size(2), (int)a.rot, (int)cache_k.size(2),
+                              cache_k.size(0) * cache_k.size(2), is_bf16(q), a.is64(), a.w_bf16(), a.interleaved, (float)a.eps, (float)a.amp, stream()),
+        "norm_rope_to_cache");
+  count();
+  return out;
+}
+
+bool pages_fit(const Tensor& table, const Tensor& lens, const Tensor& per, at::ScalarType type, const Tensor& ring, const Tensor& range, int64_t page) {
+  if (!table.is_cuda() || table.dim() != 2 || table.scalar_type() != at::kInt || (table.stride(1) != 1 && table.size(1) > 1) || page < 1) return false;
+  for (const Tensor* t : {&lens, &per})
+    if (t->dim() != 1 || t->size(0) != table.size(0) || t->device() != table.device() || !t->is_contiguous()) return false;
+  return lens.scalar_type() == at::kInt && per.scalar_type() == type && ring.dim() == 1 && ring.scalar_type() == at::kInt && ring.is_contiguous() && ring.numel() > 0 &&
+         ring.device() == table.device() && range.dim() == 1 && range.size(0) == 2 && range.scalar_type() == at::kLong && range.device() == table.device() && range.is_contiguous();
+}
+variable_list append_tokens(const Tensor& table, const Tensor& lens, const Tensor& counts, const Tensor& ring, const Tensor& range, int64_t page, int64_t max_tokens) {
+  if (!pages_fit(table, lens, counts, at::kInt, ring, range, page) || max_tokens < 0 || page > INT_MAX) return {};
+  const c10::cuda::CUDAGuard guard(table.device());
+  const int64_t n = table.size(0);
+  Tensor slots = fresh({max_tokens}, table, at::kInt), positions = fresh({max_tokens}, table, at::kInt), requests = fresh({max_tokens}, table, at::kInt),
+         offsets = fresh({n + 1}, table, at::kInt), new_lens = fresh({n}, table, at::kInt), new_range = fresh({2}, table, at::kLong), granted = fresh({n}, table, at::kBool);
+  check(rb200_paged_append(ptr<int>(table), table.stride(0), (int)table.size(1), ptr<int>(lens), ptr<int>(counts), (int)n, ptr<int>(ring), ring.numel(),
+                           ptr<long long>(range), (int)page, max_tokens, ptr<int>(slots), ptr<int>(positions), ptr<int>(requests), ptr<int>(offsets), ptr<int>(new_lens),
+                           ptr<long long>(new_range), ptr(granted), stream()),
+        "append_tokens");
+  count();
+  return {slots, positions, requests, offsets, new_lens, new_range, granted};
+}
+variable_list release_pages(const Tensor& table, const Tensor& lens, const Tensor& done, const Tensor& ring, const Tensor& range, int64_t page) {
+  if (!pages_fit(table, lens, done, at::kBool, ring, range, page) || page > INT_MAX) return {};
+  const c10::cuda::CUDAGuard guard(table.device());
+  const int64_t n = table.size(0);
+  Tensor new_lens = fresh({n}, table, at::kInt), new_range = fresh({2}, table, at::kLong);
+  check(rb200_paged_release(ptr<int>(table), table.stride(0), (int)table.size(1), ptr<int>(lens), ptr(done), (int)n, ptr<int>(ring), ring.numel(), ptr<long long>(range),
+                            (int)page, ptr<int>(new_lens), ptr<long long>(new_range), stream()),
+        "release_pages");
+  count();
+  return {new_lens, new_range};
+}
+
+Tensor paged_attention(const Tensor& q, const Tensor& cache_k, const Tensor& cache_v, const Tensor& table, const Tensor& lens, double scale, const Tensor& status) {
+  if (!q.is_cuda() || q.dim() != 3 || cache_k.dim() != 4 || !bf16_or_fp32(q) || wants_gradient({&q, &cache_k, &cache_v})) return {};
+  const int64_t n = q.size(0), heads = q.size(1), d = q.size(2), kv_heads = cache_k.size(1), unit = is_bf16(q) ? 8 : 4;
+  if (cache_v.sizes() != cache_k.sizes() || cache_k.size(3) != d || kv_heads < 1 || heads % kv_heads || cache_k.size(2) < 1 || (q.stride(2) != 1 && d > 1)) return {};
+  long long st[8] = {q.stride(0), q.stride(1)};
+  int i = 2;
+  for (const Tensor* c : {&cache_k, &cache_v}) {
+    if (c->scalar_type() != q.scalar_type() || c->device() != q.device() || c->stride(3) != 1 || !aligned16(*c)) return {};
+    for (int64_t j = 0; j < 3; ++j, ++i) {
+      st[i] = c->size(j) > 1 ? c->stride(j) : 0;  // (the stride of an axis of one element is never used)
+      if (st[i] % unit) return {};
+    }
+  }
+  if (table.dim() != 2 || table.size(0) != n || table.scalar_type() != at::kInt || (table.stride(1) != 1 && table.size(1) > 1) || table.device() != q.device() ||
+      lens.dim() != 1 || lens.size(0) != n || lens.scalar_type() != at::kInt || !lens.is_contiguous() || lens.device() != q.device())
+    return {};
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = fresh(q.sizes(), q, q.scalar_type());
+  Tensor work = fresh({(rb200_paged_attention_workspace((int)n, (int)heads, (int)kv_heads, (int)d, is_bf16(q)) + 3) / 4}, q, at::kFloat);
+  check(rb200_paged_attention(ptr(q), ptr(cache_k), ptr(cache_v), ptr<int>(table), table.stride(0), ptr<int>(lens), ptr(out), ptr(work), st, (int)n, (int)heads,
+                              (int)kv_heads, (int)d, (int)cache_k.size(2), (int)table.size(1), (int)cache_k.size(0), (float)scale, is_bf16(q), ptr<int>(status), stream()),
+        "paged_attention");
+  count(2);
+  return out;
+}
+
+struct TokenScores {
+  Tensor lp, norm, entropy, top, labels;
+};
+TokenScores token_log_probs_forward(const Tensor& x, const Tensor& targets, bool entropy, int64_t num_top, bool keep) {
+  const int64_t rows = x.size(0), v = x.size(1);
+  TokenScores r;
+  r.lp = fresh({rows}, x, at::kFloat);
+  if (keep) r.norm = fresh({rows, 2}, x, at::kFloat);
+  if (entropy) r.entropy = fresh({rows}, x, at::kFloat);
+  if (num_top) {
+    r.top = fresh({rows, num_top}, x, at::kFloat);
+    r.labels = fresh({rows, num_top}, x, at::kInt);
+  }
+  check(rb200_token_log_probs_fwd(ptr(x), x.stride(0), ptr(targets), targets.scalar_type() == at::kLong, rows, (int)v, (int)num_top, is_bf16(x), ptr<float>(r.lp),
+                                  (float*)data(r.norm), (float*)data(r.entropy), (float*)data(r.top), (int*)data(r.labels), stream()),
+        "token_log_probs");
+  count();
+  return r;
+}
+
+struct TokenLogProbs : Function<TokenLogProbs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& targets, bool entropy, int64_t num_top) {
+    TokenScores r = token_log_probs_forward(x, targets, entropy, num_top, true);
+    ctx->save_for_backward({x, targets, r.norm, r.entropy, r.labels});
+    ctx->set_materialize_grads(false);
+    variable_list out = {r.lp};
+    if (entropy) out.push_back(r.entropy);
+    if (num_top) {
+      out.push_back(r.top);
+      out.push_back(r.labels);
+      ctx->mark_non_differentiable({r.labels});
+    }
+    ctx->saved_data["num_top"] = num_top;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &targets = s[1], &norm = s[2], &entropy = s[3], &labels = s[4];
+    const int64_t num_top = ctx->saved_data["num_top"].toInt();
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor d_lp = grads[0], d_entropy = entropy.defined() ? grads[1] : Tensor(), d_top = num_top ? grads[entropy.defined() ? 2 : 1] : Tensor();
+    Tensor dx = fresh(x.sizes(), x, x.scalar_type());
+    check(rb200_token_log_probs_bwd(ptr(x), x.stride(0), ptr(targets), targets.scalar_type() == at::kLong, ptr<float>(norm), (const float*)data(entropy),
+                                    (const int*)data(labels), (const float*)data(d_lp), d_lp.defined() ? d_lp.stride(0) : 0, (const float*)data(d_entropy),
+                                    d_entropy.defined() ? d_entropy.stride(0) : 0, (const float*)data(d_top), d_top.defined() ? d_top.stride(0) : 0,
+                                    d_top.defined() ? d_top.stride(1) : 0, ptr(dx), x.size(0), (int)x.size(1), (int)num_top, is_bf16(x), stream()),
+          "token_log_probs_bwd");
+    count();
+    return {dx, Tensor(), Tensor(), Tensor()};
+  }
+};
+// log probabilities, entropy, best, labels; undefined: not asked for
+variable_list token_log_probs(const Tensor& x, const Tensor& targets, bool entropy, int64_t num_top) {
+  if (!x.is_cuda() || x.dim() != 2 || !bf16_or_fp32(x) || (x.stride(1) != 1 && x.size(1) > 1) || x.size(1) < 1 || x.size(1) > INT_MAX || targets.dim() != 1 ||
+      targets.size(0) != x.size(0) || (targets.scalar_type() != at::kInt && targets.scalar_type() != at::kLong) || targets.device() != x.device() ||
+      !targets.is_contiguous() || num_top < 0 || num_top > std::min<int64_t>(32, x.size(1)))
+    return {};
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (!wants_gradient({&x})) {
+    TokenScores r = token_log_probs_forward(x, targets, entropy, num_top, false);
+    return {r.lp, r.entropy, r.top, r.labels};
+  }
+  const variable_list out = TokenLogProbs::apply(x, targets, entropy, num_top);
+  const size_t e = entropy ? 1 : 0;
+  return {out[0], entropy ? out[1] : Tensor(), num_top ? out[1 + e] : Tensor(), num_top ? out[2 + e] : Tensor()};
+}
+
 // ---- the Python side: positional arguments, checked for number and type
 struct Args {
   PyObject* const* args;
@@ -489,6 +775,67 @@ PyObject* py_flash(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return enter<4>(args, n, [](Args a) { return CrossEntropy::apply(a.tensor(0), a.tensor(1), a.number(2), a.truth(3)); });
 }
+PyObject* wrap_or_none(const Tensor& t) {
+  if (!t.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(t);
+}
+// a tuple, None in the place of undefined ones; None for an empty list
+template <int N, typename Call>
+PyObject* enter_list(PyObject* const* args, Py_ssize_t n, Call call) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == N, "expected ", N, " arguments, got ", (long)n);
+  const variable_list r = call(Args{args});
+  if (r.empty()) Py_RETURN_NONE;
+  PyObject* t = PyTuple_New((Py_ssize_t)r.size());
+  if (!t) throw python_error();
+  for (size_t i = 0; i < r.size(); ++i) {
+    PyObject* o = wrap_or_none(r[i]);
+    if (!o) {
+      Py_DECREF(t);
+      throw python_error();
+    }
+    PyTuple_SET_ITEM(t, (Py_ssize_t)i, o);
+  }
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+template <int N, typename Call>
+PyObject* enter_opt(PyObject* const* args, Py_ssize_t n, Call call) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == N, "expected ", N, " arguments, got ", (long)n);
+  return wrap_or_none(call(Args{args}));
+  END_HANDLE_TH_ERRORS
+}
+RopeArgs rope_args(const Args& a, int i) {  // positions, frequencies, q_scale, k_scale, eps, interleaved, amplitude
+  RopeArgs r;
+  auto opt = [&](int j) { return a.args[j] == Py_None ? Tensor() : a.tensor(j); };
+  r.positions = opt(i);
+  r.frequencies = opt(i + 1);
+  r.wq = opt(i + 2);
+  r.wk = opt(i + 3);
+  r.eps = a.number(i + 4);
+  r.interleaved = a.truth(i + 5);
+  r.amp = a.number(i + 6);
+  return r;
+}
+PyObject* py_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return enter_list<9>(args, n, [](Args a) { return norm_rope(a.tensor(0), a.tensor(1), rope_args(a, 2)); });
+}
+PyObject* py_norm_rope_to_cache(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return enter_opt<13>(args, n, [](Args a) { return norm_rope_to_cache(a.tensor(0), a.tensor(1), a.tensor(2), a.tensor(3), a.tensor(4), a.tensor(5), rope_args(a, 6)); });
+}
+PyObject* py_append_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return enter_list<7>(args, n, [](Args a) { return append_tokens(a.tensor(0), a.tensor(1), a.tensor(2), a.tensor(3), a.tensor(4), a.integer(5), a.integer(6)); });
+}
+PyObject* py_release_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return enter_list<6>(args, n, [](Args a) { return release_pages(a.tensor(0), a.tensor(1), a.tensor(2), a.tensor(3), a.tensor(4), a.integer(5)); });
+}
+PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return enter_opt<7>(args, n, [](Args a) { return paged_attention(a.tensor(0), a.tensor(1), a.tensor(2), a.tensor(3), a.tensor(4), a.number(5), a.tensor(6)); });
+}
+PyObject* py_token_log_probs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return enter_list<4>(args, n, [](Args a) { return token_log_probs(a.tensor(0), a.tensor(1), a.truth(2), a.integer(3)); });
+}
 PyObject* py_set_allocator(PyObject*, PyObject* hook) {  // the caller keeps the hook alive until it is replaced
   allocator.store(hook == Py_None ? nullptr : hook, std::memory_order_release);
   Py_RETURN_NONE;
@@ -506,6 +853,12 @@ PyMethodDef methods[] = {
     fast<py_conv_module>("conv_module", "(x, filt, bias, gamma, beta, running_mean, running_var, row_batch, row_pos, lens, eps, momentum) -> z"),
     fast<py_flash>("flash", "(q, k, v, k_lens, causal, scale, p_drop, seed, status) -> o"),
     fast<py_cross_entropy>("cross_entropy", "(logits, targets, smoothing, grad_only) -> loss"),
+    fast<py_norm_rope>("norm_rope", "(q, k, positions, frequencies, q_scale, k_scale, eps, interleaved, amplitude) -> (q, k) or None: not a plain case"),
+    fast<py_norm_rope_to_cache>("norm_rope_to_cache", "(q, k, v, k_cache, v_cache, slots, positions, frequencies, q_scale, k_scale, eps, interleaved, amplitude) -> q or None"),
+    fast<py_append_tokens>("append_tokens", "(block_table, lengths, counts, free_pages, free_range, page_size, max_tokens) -> tuple or None"),
+    fast<py_release_pages>("release_pages", "(block_table, lengths, finished, free_pages, free_range, page_size) -> tuple or None"),
+    fast<py_paged_attention>("paged_attention", "(q, k_cache, v_cache, block_table, lengths, scale, status) -> out or None"),
+    fast<py_token_log_probs>("token_log_probs", "(logits, targets, entropy, num_top) -> (log_probs, entropy, top_log_probs, top_labels) or None"),
     {"set_allocator", py_set_allocator, METH_O, "(hook or None): allocate through hook(like, shape, type); for debugging"},
     {"launches", py_launches, METH_NOARGS, "kernels launched by the nodes so far"},
     {nullptr, nullptr, 0, nullptr}};
