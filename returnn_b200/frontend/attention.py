@@ -295,14 +295,81 @@ def _rope_base(head_dim: Dim) -> float:
     return 10_000 ** (1 - 2 / head_dim.dimension)
 
 
+def _rotary_init(self, qk_norm: bool, rope: Optional[dict]):
+    """
+    Options of the rotary modules beyond the reference's. ``qk_norm``: an RMS norm of each head of the queries and keys before the rotation (``q_norm``, ``k_norm``
+    with one scale of ``key_dim_per_head`` each). ``rope``: ``rotary_dim`` (features of a head that are rotated, default all), ``base``, ``scaling``
+    (see :func:`returnn_b200.ops.norm_rope.rope_frequencies`) and ``interleaved`` (pairs ``(2i, 2i + 1)``, the default, or ``(i, i + rotary_dim / 2)``). With either of them
+    norm and rotation of queries and keys are one kernel in each direction, in 32 bits; ``rope={}`` asks for that without another option.
+    """
+    self.q_norm = self.k_norm = None
+    if qk_norm:
+        from .normalization import RMSNorm
+
+        self.q_norm = RMSNorm(self.key_dim_per_head)
+        self.k_norm = RMSNorm(self.key_dim_per_head)
+    if rope is None and qk_norm:
+        rope = {}
+    self.rope = None
+    if rope is not None:
+        from ..ops.norm_rope import rope_frequencies
+
+        rope = dict(rope)
+        interleaved = bool(rope.pop("interleaved", True))
+        freq, amplitude = rope_frequencies(rope.pop("rotary_dim", self.key_dim_per_head.dimension), base=rope.pop("base", 10_000.0), scaling=rope.pop("scaling", None))
+        if rope:
+            raise TypeError("%s: unexpected rope options %r" % (self, sorted(rope)))
+        if 2 * len(freq) > self.key_dim_per_head.dimension:
+            raise ValueError("%s: rotary dim %i of a head dim of %i" % (self, 2 * len(freq), self.key_dim_per_head.dimension))
+        self.rope = dict(frequencies=freq, interleaved=interleaved, amplitude=amplitude)
+
+
+def _rotary_frequencies(self, device) -> torch.Tensor:
+    freq = self.rope["frequencies"]
+    if freq.device != torch.device(device):
+        self.rope["frequencies"] = freq = freq.to(device)
+    return freq
+
+
+def _rotary_norm_rope(self, q: Tensor, k: Tensor, *, axis: Dim, offset: int = 0) -> Tuple[Tensor, Tensor]:
+    from ..ops.norm_rope import norm_rope
+
+    batch_dims = [d for d in q.dims if d not in (axis, self.num_heads, self.key_dim_per_head)]
+    tokens = batch_dims + ([axis] if axis != single_step_dim else [])
+    qr, kr = (x.copy_compatible_to_dims_raw(tokens + [self.num_heads, self.key_dim_per_head]) for x in (q, k))
+    if not tokens:
+        qr, kr = qr.unsqueeze(0), kr.unsqueeze(0)
+    if axis == single_step_dim:
+        positions = torch.full(qr.shape[:-2], offset, dtype=torch.int32, device=qr.device)
+    else:
+        positions = torch.arange(offset, offset + qr.shape[-3], dtype=torch.int32, device=qr.device)
+    norms = dict(q_scale=self.q_norm.scale.raw_tensor, k_scale=self.k_norm.scale.raw_tensor, eps=self.q_norm.eps) if self.q_norm is not None else {}
+    qr, kr = norm_rope(qr, kr, positions, _rotary_frequencies(self, qr.device), interleaved=self.rope["interleaved"], amplitude=self.rope["amplitude"], **norms)
+    if not tokens:
+        qr, kr = qr.squeeze(0), kr.squeeze(0)
+    dims = tokens + [self.num_heads, self.key_dim_per_head]
+    return wrap(qr, dims, feature_dim=self.key_dim_per_head), wrap(kr, dims, feature_dim=self.key_dim_per_head)
+
+
 class RotaryPosSelfAttention(SelfAttention):
     """self-attention with rotary position embedding (RoPE) on q and k"""
 
+    def __init__(self, in_dim: Dim, proj_dim: Optional[Dim], *, qk_norm: bool = False, rope: Optional[dict] = None, **kwargs):
+        """
+        :param qk_norm: RMS norm of each head of q and k before the rotation
+        :param rope: options of the rotation, see :func:`_rotary_init`
+        """
+        super().__init__(in_dim, proj_dim, **kwargs)
+        _rotary_init(self, qk_norm, rope)
+
     def __call__(self, source: Tensor, *, axis: Dim) -> Tensor:
         q, k, v = self.forward_qkv(source)
-        pos_enc = sinusoidal_positional_encoding(spatial_dim=axis, feat_dim=self.key_dim_per_head, base=_rope_base(self.key_dim_per_head), device=source.device)
-        q = _apply_rope(q, pos_enc, self.key_dim_per_head)
-        k = _apply_rope(k, pos_enc, self.key_dim_per_head)
+        if self.rope is not None:
+            q, k = _rotary_norm_rope(self, q, k, axis=axis)
+        else:
+            pos_enc = sinusoidal_positional_encoding(spatial_dim=axis, feat_dim=self.key_dim_per_head, base=_rope_base(self.key_dim_per_head), device=source.device)
+            q = _apply_rope(q, pos_enc, self.key_dim_per_head)
+            k = _apply_rope(k, pos_enc, self.key_dim_per_head)
         kv_axis = Dim(None, name="%s-kv" % axis.name)
         k, _ = _replace(k, axis, kv_axis)
         v, _ = _replace(v, axis, kv_axis)
@@ -312,17 +379,30 @@ class RotaryPosSelfAttention(SelfAttention):
 class RotaryPosCausalSelfAttention(CausalSelfAttention):
     """causal self-attention with RoPE"""
 
+    def __init__(self, in_dim: Dim, proj_dim: Optional[Dim], *, qk_norm: bool = False, rope: Optional[dict] = None, **kwargs):
+        """
+        :param qk_norm: RMS norm of each head of q and k before the rotation
+        :param rope: options of the rotation, see :func:`_rotary_init`
+        """
+        super().__init__(in_dim, proj_dim, **kwargs)
+        _rotary_init(self, qk_norm, rope)
+
     def __call__(self, source: Tensor, *, axis: Dim, state: Optional[CausalSelfAttentionState] = None):
         q, k, v = self.forward_qkv(source)
+        offset = 0
         if axis == single_step_dim:
             assert state
             offset = state.accum_axis.get_dim_value() if state.accum_axis.dimension != 0 else 0
-            pos_enc = sinusoidal_positional_encoding(spatial_dim=single_step_dim, offset=offset, feat_dim=self.key_dim_per_head,
-                                                     base=_rope_base(self.key_dim_per_head), device=source.device)
+        if self.rope is not None:
+            q, k = _rotary_norm_rope(self, q, k, axis=axis, offset=int(offset))
         else:
-            pos_enc = sinusoidal_positional_encoding(spatial_dim=axis, feat_dim=self.key_dim_per_head, base=_rope_base(self.key_dim_per_head), device=source.device)
-        q = _apply_rope(q, pos_enc, self.key_dim_per_head)
-        k = _apply_rope(k, pos_enc, self.key_dim_per_head)
+            if axis == single_step_dim:
+                pos_enc = sinusoidal_positional_encoding(spatial_dim=single_step_dim, offset=offset, feat_dim=self.key_dim_per_head,
+                                                         base=_rope_base(self.key_dim_per_head), device=source.device)
+            else:
+                pos_enc = sinusoidal_positional_encoding(spatial_dim=axis, feat_dim=self.key_dim_per_head, base=_rope_base(self.key_dim_per_head), device=source.device)
+            q = _apply_rope(q, pos_enc, self.key_dim_per_head)
+            k = _apply_rope(k, pos_enc, self.key_dim_per_head)
         k, v, hist_dim, new_state, causal_dim = _causal_self_att_step(k, v, axis=axis, state=state, self=self)
         output = self.attention(q, k, v, kv_axis=hist_dim, causal_query_spatial_dim=causal_dim)
         return output, new_state

@@ -6,13 +6,13 @@ CTC backend semantics returnn/torch/frontend/_backend.py:775-869.
 """
 
 from __future__ import annotations
-from typing import Optional, Tuple, Union
+from typing import NamedTuple, Optional, Tuple, Union
 import torch
 import torch.nn.functional as F
 from ..tensor import Tensor, Dim, batch_dim
 from ._utils import wrap, axis_of
 
-__all__ = ["cross_entropy", "softmax_cross_entropy_smoothed_grad", "ctc_loss", "ctc_best_path", "ctc_durations_from_path", "ctc_no_label_loop_blank_durations_from_path",
+__all__ = ["cross_entropy", "softmax_cross_entropy_smoothed_grad", "token_log_probs", "TokenLogProbs", "ctc_loss", "ctc_best_path", "ctc_durations_from_path", "ctc_no_label_loop_blank_durations_from_path",
            "ctc_greedy_decode", "edit_distance", "mse_loss", "binary_cross_entropy"]
 
 
@@ -93,6 +93,54 @@ def softmax_cross_entropy_smoothed_grad(*, logits: Tensor, target: Tensor, axis:
     loss, best = res
     best_t = Tensor("argmax", dims=rest, dtype=target.dtype, sparse_dim=axis, raw_tensor=best.reshape(shape).to(tgt.dtype))
     return wrap(loss.reshape(shape), rest), best_t
+
+
+class TokenLogProbs(NamedTuple):
+    """what :func:`token_log_probs` returns; None: not asked for"""
+
+    log_probs: Tensor
+    entropy: Optional[Tensor] = None
+    top_log_probs: Optional[Tensor] = None
+    top_labels: Optional[Tensor] = None
+    top_dim: Optional[Dim] = None
+
+
+def token_log_probs(*, logits: Tensor, target: Tensor, axis: Dim, entropy: bool = False, num_top: int = 0) -> TokenLogProbs:
+    """
+    What scoring, rescoring and sequence training with a language model read off its output layer, in one pass over the logits and differentiable in them::
+
+        log_prob = rf.log_softmax(logits, axis=axis)
+        log_probs = rf.gather(log_prob, indices=target, axis=axis)
+        entropy = -rf.reduce_sum(rf.exp(log_prob) * log_prob, axis=axis)
+        top_log_probs, top_labels, top_dim = rf.top_k(log_prob, axis=axis, k=num_top)
+
+    On the GPU this is one kernel forward and one backward (:mod:`returnn_b200.ops.token_log_probs`); the log-probabilities of all labels are never
+    materialised.
+
+    :param logits: [..., axis]
+    :param target: sparse, sparse_dim == axis; a label outside 0 .. axis size - 1 has log probability 0 and no gradient
+    :param entropy: also the entropy of the distributions
+    :param num_top: also that many best labels (the lowest first among equal ones), at most 32
+    """
+    from ..ops import token_log_probs as _tlp
+
+    if target.sparse_dim is not None and target.sparse_dim != axis:
+        raise ValueError("token_log_probs: the labels of %s are %s, the logits are over %s" % (target, target.sparse_dim, axis))
+    rest = [d for d in logits._dims if d != axis]
+    raw = logits.copy_compatible_to_dims_raw(rest + [axis])
+    tgt = target.copy_compatible_to_dims_raw(rest)
+    shape = list(raw.shape[:-1])
+    if list(tgt.shape) != shape:
+        tgt = tgt.expand(*shape)
+    res = _tlp.token_log_probs(raw.reshape(-1, raw.shape[-1]), tgt.reshape(-1).to(raw.device), entropy=entropy, num_top=num_top)
+    out = TokenLogProbs(wrap(res.log_probs.reshape(shape), rest))
+    if entropy:
+        out = out._replace(entropy=wrap(res.entropy.reshape(shape), rest))
+    if num_top:
+        top_dim = Dim(num_top, name="top")
+        labels = Tensor("top_labels", dims=rest + [top_dim], dtype=target.dtype, sparse_dim=axis, raw_tensor=res.top_labels.reshape(shape + [num_top]).to(tgt.dtype))
+        out = out._replace(top_log_probs=wrap(res.top_log_probs.reshape(shape + [num_top]), rest + [top_dim]), top_labels=labels, top_dim=top_dim)
+    return out
 
 
 def mse_loss(estimated: Tensor, target: Tensor) -> Tensor:
