@@ -130,6 +130,31 @@ Tensor fresh(at::IntArrayRef shape, const Tensor& like, at::ScalarType type) {
   }
   return at::empty(shape, like.options().dtype(type));
 }
+struct Wanted {
+  Tensor* to;
+  c10::DimVector shape;
+  at::ScalarType type;
+};
+// Several small results of one call in one allocation: an allocation of its own is a microsecond on the host for each, as long as their kernel runs. They are tensors
+// of their own at 64-byte boundaries of one storage.
+void fresh_small(const Tensor& like, std::initializer_list<Wanted> wanted) {
+  if (allocator.load(std::memory_order_acquire)) {  // the debugger wants each by itself
+    for (const Wanted& w : wanted) *w.to = fresh(w.shape, like, w.type);
+    return;
+  }
+  auto bytes = [](const Wanted& w) { return (c10::multiply_integers(w.shape) * (int64_t)c10::elementSize(w.type) + 63) / 64 * 64; };
+  int64_t total = 0;
+  for (const Wanted& w : wanted) total += bytes(w);
+  const c10::Storage storage = at::empty({total}, like.options().dtype(at::kByte)).storage();
+  int64_t at = 0;
+  for (const Wanted& w : wanted) {
+    *w.to = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(storage), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(w.type));
+    c10::TensorImpl* impl = w.to->unsafeGetTensorImpl();
+    impl->set_storage_offset(at / (int64_t)c10::elementSize(w.type));
+    impl->set_sizes_contiguous(w.shape);
+    at += bytes(w);
+  }
+}
 Tensor fresh_like(const Tensor& t) { return fresh(t.sizes(), t, t.scalar_type()); }  // (contiguous)
 
 // ---- layer norm, RMS norm
@@ -612,8 +637,14 @@ variable_list append_tokens(const Tensor& table, const Tensor& lens, const Tenso
   if (!pages_fit(table, lens, counts, at::kInt, ring, range, page) || max_tokens < 0 || page > INT_MAX) return {};
   const c10::cuda::CUDAGuard guard(table.device());
   const int64_t n = table.size(0);
-  Tensor slots = fresh({max_tokens}, table, at::kInt), positions = fresh({max_tokens}, table, at::kInt), requests = fresh({max_tokens}, table, at::kInt),
-         offsets = fresh({n + 1}, table, at::kInt), new_lens = fresh({n}, table, at::kInt), new_range = fresh({2}, table, at::kLong), granted = fresh({n}, table, at::kBool);
+  Tensor slots, positions, requests, offsets, new_lens, new_range, granted;
+  fresh_small(table, {{&slots, {max_tokens}, at::kInt},
+                      {&positions, {max_tokens}, at::kInt},
+                      {&requests, {max_tokens}, at::kInt},
+                      {&offsets, {n + 1}, at::kInt},
+                      {&new_lens, {n}, at::kInt},
+                      {&new_range, {2}, at::kLong},
+                      {&granted, {n}, at::kBool}});
   check(rb200_paged_append(ptr<int>(table), table.stride(0), (int)table.size(1), ptr<int>(lens), ptr<int>(counts), (int)n, ptr<int>(ring), ring.numel(),
                            ptr<long long>(range), (int)page, max_tokens, ptr<int>(slots), ptr<int>(positions), ptr<int>(requests), ptr<int>(offsets), ptr<int>(new_lens),
                            ptr<long long>(new_range), ptr(granted), stream()),
@@ -625,7 +656,8 @@ variable_list release_pages(const Tensor& table, const Tensor& lens, const Tenso
   if (!pages_fit(table, lens, done, at::kBool, ring, range, page) || page > INT_MAX) return {};
   const c10::cuda::CUDAGuard guard(table.device());
   const int64_t n = table.size(0);
-  Tensor new_lens = fresh({n}, table, at::kInt), new_range = fresh({2}, table, at::kLong);
+  Tensor new_lens, new_range;
+  fresh_small(table, {{&new_lens, {n}, at::kInt}, {&new_range, {2}, at::kLong}});
   check(rb200_paged_release(ptr<int>(table), table.stride(0), (int)table.size(1), ptr<int>(lens), ptr(done), (int)n, ptr<int>(ring), ring.numel(), ptr<long long>(range),
                             (int)page, ptr<int>(new_lens), ptr<long long>(new_range), stream()),
         "release_pages");
@@ -665,13 +697,12 @@ struct TokenScores {
 TokenScores token_log_probs_forward(const Tensor& x, const Tensor& targets, bool entropy, int64_t num_top, bool keep) {
   const int64_t rows = x.size(0), v = x.size(1);
   TokenScores r;
-  r.lp = fresh({rows}, x, at::kFloat);
-  if (keep) r.norm = fresh({rows, 2}, x, at::kFloat);
-  if (entropy) r.entropy = fresh({rows}, x, at::kFloat);
-  if (num_top) {
-    r.top = fresh({rows, num_top}, x, at::kFloat);
-    r.labels = fresh({rows, num_top}, x, at::kInt);
-  }
+  Tensor none;
+  fresh_small(x, {{&r.lp, {rows}, at::kFloat},
+                  {keep ? &r.norm : &none, {keep ? rows : 0, 2}, at::kFloat},
+                  {entropy ? &r.entropy : &none, {entropy ? rows : 0}, at::kFloat},
+                  {num_top ? &r.top : &none, {rows, num_top}, at::kFloat},
+                  {num_top ? &r.labels : &none, {rows, num_top}, at::kInt}});
   check(rb200_token_log_probs_fwd(ptr(x), x.stride(0), ptr(targets), targets.scalar_type() == at::kLong, rows, (int)v, (int)num_top, is_bf16(x), ptr<float>(r.lp),
                                   (float*)data(r.norm), (float*)data(r.entropy), (float*)data(r.top), (int*)data(r.labels), stream()),
         "token_log_probs");
