@@ -553,42 +553,49 @@ std::pair<Tensor, Tensor> norm_rope_forward(const Tensor& q, const Tensor& q3, c
   return {out_q, out_k};
 }
 
+struct RopeSaved : torch::CustomClassHolder {  // one entry for what is not a tensor: an entry each costs a microsecond on the host both ways
+  double eps, amp;
+  bool interleaved;
+  int64_t count, rot;
+  c10::DimVector q, k;
+};
 struct NormRope : Function<NormRope> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& wq_, const OptTensor& wk_, const RopeArgs& a) {
     const Tensor q3 = token_rows(q), k3 = token_rows(k), wq = wq_.has_value() ? wq_->contiguous() : Tensor(), wk = wk_.has_value() ? wk_->contiguous() : Tensor();
     auto [out_q, out_k] = norm_rope_forward(q, q3, k, k3, a, wq, wk);
     // without a norm the gradient is a rotation back: the inputs are not kept
     ctx->save_for_backward({wq.defined() ? q3 : Tensor(), wq.defined() ? k3 : Tensor(), a.positions, a.frequencies, wq, wk});
-    auto& d = ctx->saved_data;
-    d["eps"] = a.eps;
-    d["amp"] = a.amp;
-    d["interleaved"] = a.interleaved;
-    d["count"] = a.count;
-    d["rot"] = a.rot;
-    d["q"] = q.sizes().vec();
-    d["k"] = k.sizes().vec();
+    auto d = c10::make_intrusive<RopeSaved>();
+    d->eps = a.eps;
+    d->amp = a.amp;
+    d->interleaved = a.interleaved;
+    d->count = a.count;
+    d->rot = a.rot;
+    d->q = q.sizes();
+    d->k = k.sizes();
+    ctx->saved_data["rope"] = c10::IValue::make_capsule(std::move(d));
     return {out_q, out_k};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
     const Tensor &q3 = s[0], &k3 = s[1], &positions = s[2], &frequencies = s[3], &wq = s[4], &wk = s[5];
-    auto& d = ctx->saved_data;
+    const auto held = ctx->saved_data["rope"].toCapsule();
+    const RopeSaved& d = static_cast<const RopeSaved&>(*held);
     const c10::cuda::CUDAGuard guard(grads[0].device());
     const Tensor dq = token_rows(grads[0]), dk = token_rows(grads[1]);
     const int64_t dim = dq.size(2);
-    Tensor gq = fresh(d["q"].toIntVector(), dq, dq.scalar_type()), gk = fresh(d["k"].toIntVector(), dq, dq.scalar_type()), part, dwq, dwk;
+    Tensor gq = fresh(d.q, dq, dq.scalar_type()), gk = fresh(d.k, dq, dq.scalar_type()), part, dwq, dwk;
     if (wq.defined()) {
       part = fresh({rb200_norm_rope_parts(), 2 * dim}, dq, at::kFloat);
-      dwq = fresh_like(wq);
-      dwk = fresh_like(wk);
+      fresh_small(dq, {{&dwq, {dim}, wq.scalar_type()}, {&dwk, {dim}, wk.scalar_type()}});
     }
     const bool norm = wq.defined();
     const long long st[8] = {dq.stride(0), dq.stride(1), dk.stride(0), dk.stride(1), norm ? q3.stride(0) : 0, norm ? q3.stride(1) : 0, norm ? k3.stride(0) : 0,
                              norm ? k3.stride(1) : 0};
-    check(rb200_norm_rope_bwd(ptr(dq), ptr(dk), data(q3), data(k3), data(positions), d["count"].toInt(), (const float*)data(frequencies), data(wq), data(wk), ptr(gq), ptr(gk),
-                              (float*)data(part), data(dwq), data(dwk), st, dq.size(0), (int)dq.size(1), (int)dk.size(1), (int)dim, (int)d["rot"].toInt(), is_bf16(dq),
-                              positions.defined() && positions.scalar_type() == at::kLong, norm && is_bf16(wq), d["interleaved"].toBool(), (float)d["eps"].toDouble(),
-                              (float)d["amp"].toDouble(), stream()),
+    check(rb200_norm_rope_bwd(ptr(dq), ptr(dk), data(q3), data(k3), data(positions), d.count, (const float*)data(frequencies), data(wq), data(wk), ptr(gq), ptr(gk),
+                              (float*)data(part), data(dwq), data(dwk), st, dq.size(0), (int)dq.size(1), (int)dk.size(1), (int)dim, (int)d.rot, is_bf16(dq),
+                              positions.defined() && positions.scalar_type() == at::kLong, norm && is_bf16(wq), d.interleaved, (float)d.eps,
+                              (float)d.amp, stream()),
           "norm_rope_bwd");
     count(norm ? 2 : 1);
     return {gq, gk, dwq, dwk, Tensor()};
