@@ -12,6 +12,7 @@
 // Backward: one pass, p from the maximum and the sum; the labels that have a gradient of their own are written once more at the end.
 #include "class_rows.cuh"
 #include "packed_f32.cuh"
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -24,7 +25,7 @@ constexpr int kBack = 256;  // threads of the backward pass
 constexpr int kMaxTop = 32;
 constexpr int kCand = 512;  // logits that are ranked
 // Up to this many best the bound comes from 32 groups of threads (32 shuffles; 12 of 32 are reached by 15 logits on the average), beyond from the threads themselves (a search bit by
-// bit, about a microsecond; 32 of 32 groups would be reached by 130). 1500 rows x 10001 fp32, 32 best: 60 and 31 us
+// bit, about a microsecond; 32 of 32 groups would be reached by 130). 1500 rows x 10001 fp32, groups and threads: 8 best 18.1 and 18.8 us, 16 best 23.3 and 22.1, 32 best 56 and 29
 constexpr int kFewTop = 12;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -277,7 +278,7 @@ __device__ __forceinline__ float log_prob(float x, float2 norm) {
 
 // kBatch: chunks of 16 bytes that a thread has in flight
 template <int kThreads, bool kBf16, bool kEntropy, bool kTop, int kBatch>
-__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 6 : 1)
+__global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : kBatch == 8 ? 4 : 1536 / kThreads)
 forward_kernel(const Args a) {
   constexpr int kN = Chunk<kBf16>::kN, kWarps = kThreads / 32;
   __shared__ float sh_m[kWarps], sh_s[kWarps], sh_w[kWarps];
@@ -364,9 +365,10 @@ forward_kernel(const Args a) {
         g = __reduce_max_sync(0xffffffffu, g);
         if (lane == 0) best.group[warp] = g;
       } else {
+        constexpr int kOf = kThreads / 32;  // threads of a group
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if ((lane & 7) == 0) best.group[warp * 4 + (lane >> 3)] = g;
+        for (int o = 1; o < kOf; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if (lane % kOf == 0) best.group[threadIdx.x / kOf] = g;
       }
     } else {
       best.key[threadIdx.x] = key;
@@ -437,9 +439,10 @@ struct BackArgs {
   const int* top_label;
   void* dx;
   int target64, v, top;
+  int part;  // labels of a CTA's share of a row, a multiple of 8
 };
 
-// kTop: the best labels have gradients too. kLastFirst: rows from the last one on.
+// kTop: the best labels have gradients too. kLastFirst: rows from the last one on. Block (row, share of its labels); share 0 has those outside the chunks too.
 template <bool kBf16, bool kEntropy, bool kTop, bool kLastFirst>
 __global__ void __launch_bounds__(kBack)
 backward_kernel(const BackArgs a) {
@@ -478,6 +481,9 @@ backward_kernel(const BackArgs a) {
   const int head_in = row_head(a.x, base, a.v, kBf16 ? 2 : 4), head_out = row_head(a.dx, out, a.v, kBf16 ? 2 : 4);
   const int head = head_in == head_out ? head_in : a.v;  // (rows that are aligned differently: single elements)
   const int v8 = head + ((a.v - head) & ~7);
+  const int lo = (int)min((int64_t)v8, head + (int64_t)blockIdx.y * a.part), hi = (int)min((int64_t)v8, (int64_t)lo + a.part);
+  const bool outside = blockIdx.y == 0;
+  auto mine = [&](int c) { return c >= head && c < v8 ? c >= lo && c < hi : outside; };
   auto put = [&](int64_t c, float d) {
     if (kBf16) reinterpret_cast<__nv_bfloat16*>(a.dx)[out + c] = __float2bfloat16(d);
     else reinterpret_cast<float*>(a.dx)[out + c] = d;
@@ -488,7 +494,7 @@ backward_kernel(const BackArgs a) {
     const float at0 = -(all + ge * h);
     const uint64_t offset = two(at0, at0);
 #pragma unroll 4
-    for (int64_t c = head + (int)threadIdx.x * 8; c < v8; c += kBack * 8) {
+    for (int64_t c = lo + (int)threadIdx.x * 8; c < hi; c += kBack * 8) {
       constexpr int kN = Chunk<kBf16>::kN;
       Chunk<kBf16> u[8 / kN];
 #pragma unroll
@@ -510,23 +516,23 @@ backward_kernel(const BackArgs a) {
       store8(a.dx, out + c, d, kBf16);
     }
   } else {
-    for (int64_t c = head + (int)threadIdx.x * 8; c < v8; c += kBack * 8)
+    for (int64_t c = lo + (int)threadIdx.x * 8; c < hi; c += kBack * 8)
       for (int k = 0; k < 8; ++k) put(c + k, of(ld(a.x, base + c + k, kBf16)));
   }
-  for (int i = threadIdx.x; i < a.v - (v8 - head); i += kBack) {
+  for (int i = threadIdx.x; outside && i < a.v - (v8 - head); i += kBack) {
     const int c = i < head ? i : i + (v8 - head);
     put(c, of(ld(a.x, base + c, kBf16)));
   }
   if (!kTop) {
     // the target's entry again, by the thread that wrote it
-    if (y >= 0) {
+    if (y >= 0 && mine((int)y)) {
       const int c = (int)y;
-      const int who = c >= head && c < v8 ? (c - head) / 8 % kBack : (c < head ? c : c - (v8 - head)) % kBack;
+      const int who = c >= head && c < v8 ? (c - lo) / 8 % kBack : (c < head ? c : c - (v8 - head)) % kBack;
       if ((int)threadIdx.x == who) put(c, own + of(ld(a.x, base + c, kBf16)));
     }
   } else {
     __syncthreads();
-    if ((int)threadIdx.x <= a.top && label[threadIdx.x] >= 0) {
+    if ((int)threadIdx.x <= a.top && label[threadIdx.x] >= 0 && mine(label[threadIdx.x])) {
       const int c = label[threadIdx.x];
       float sum = 0.f;
       bool first = true;
@@ -553,20 +559,27 @@ RB_EXPORT int rb200_token_log_probs_fwd(const void* x, long long pitch, const vo
   Args a = {};
   a.x = x; a.pitch = pitch; a.target = target; a.target64 = target64; a.v = v; a.top = top; a.lp = lp; a.norm = norm; a.entropy = entropy; a.top_lp = top_lp;
   a.top_label = top_label;
-  // few rows leave most of the threads to a row of many labels
-  const bool wide = rows <= 2 * 148 && v >= 8192;
-  auto pick = [&](auto threads, auto b) {
-    constexpr int kT = decltype(threads)::value;
+  // Threads of a row and 16-byte pieces that each has under way. Many rows: 128, 12 rows on an SM, where the latencies of one row's end are hidden best (bf16, us with 128
+  // and 256: 6001 x 32000 without the best 70.1 and 70.8, 8 best 89 and 94; 1500 x 10001 fp32, 8 best 18.1 and 20.8). Fewer do not fill the SMs so: 256 (850 x 32000 fp32,
+  // 32 best: 41.1 and 31.7), and twice the pieces where four rows on an SM are all (500 x 32000: 12.9, with more pieces 9.6; 486 x 128000, 5 best: 49.3 and 36.0). With
+  // two rows on an SM or fewer, 1024 threads for many labels (16 x 32000, 5 best: 8.2 with 256, 6.9; 4 x 128000 fp32, 8 best: 23.0 and 12.5; but 62 x 10001: 3.5 and 4.5).
+  const int way = rows >= 8 * 148 ? 0 : v < 8192 || rows > 4 * 148 ? 1 : rows > 2 * 148 || v < 16384 ? 2 : 3;
+  auto pick = [&](auto threads, auto batch, auto b) {
+    constexpr int kT = decltype(threads)::value, kP = decltype(batch)::value;
     constexpr bool kB = decltype(b)::value;
-    return entropy ? (top ? forward_kernel<kT, kB, true, true, 4> : forward_kernel<kT, kB, true, false, 4>)
-                   : (top ? forward_kernel<kT, kB, false, true, 4> : forward_kernel<kT, kB, false, false, 4>);
+    return entropy ? (top ? forward_kernel<kT, kB, true, true, kP> : forward_kernel<kT, kB, true, false, kP>)
+                   : (top ? forward_kernel<kT, kB, false, true, kP> : forward_kernel<kT, kB, false, false, kP>);
   };
-  using Few = std::integral_constant<int, 256>;
-  using Many = std::integral_constant<int, 1024>;
-  const std::true_type yes;
-  const std::false_type no;
-  auto kernel = bf16 ? (wide ? pick(Many(), yes) : pick(Few(), yes)) : (wide ? pick(Many(), no) : pick(Few(), no));
-  rb_launch_pdl(kernel, dim3((unsigned)rows), dim3(wide ? 1024 : 256), 0, stream, a);
+  auto of_type = [&](auto b) {
+    const std::integral_constant<int, 4> four;
+    const std::integral_constant<int, 8> eight;
+    if (way == 0) return pick(std::integral_constant<int, 128>(), four, b);
+    if (way == 1) return pick(std::integral_constant<int, 256>(), four, b);
+    if (way == 2) return pick(std::integral_constant<int, 256>(), eight, b);
+    return pick(std::integral_constant<int, 1024>(), four, b);
+  };
+  auto kernel = bf16 ? of_type(std::true_type()) : of_type(std::false_type());
+  rb_launch_pdl(kernel, dim3((unsigned)rows), dim3(way == 0 ? 128 : way == 3 ? 1024 : 256), 0, stream, a);
   return rb_check_launch("token_log_probs_fwd");
 }
 
@@ -591,6 +604,9 @@ RB_EXPORT int rb200_token_log_probs_bwd(const void* x, long long pitch, const vo
                               : (last_first ? backward_kernel<kB, false, false, true> : backward_kernel<kB, false, false, false>));
   };
   auto kernel = bf16 ? pick(std::true_type()) : pick(std::false_type());
-  rb_launch_pdl(kernel, dim3((unsigned)rows), dim3(kBack), 0, stream, a);
+  // few rows: shares of a row, as long as a thread has two chunks of 8 (25 x 128000 bf16, both passes: 28.1 us with whole rows, 13.9)
+  const long long shares = std::max(1LL, std::min(4 * 148 / rows, (long long)v / (kBack * 16)));
+  a.part = (int)(((v + shares - 1) / shares + 7) / 8 * 8);
+  rb_launch_pdl(kernel, dim3((unsigned)rows, (unsigned)shares), dim3(kBack), 0, stream, a);
   return rb_check_launch("token_log_probs_bwd");
 }
