@@ -8,7 +8,7 @@
 // Forward: one CTA per row, one pass with a running maximum, sum and sum of exp(z) z; the logits are read once. A label costs an exponential and, by packed
 // arithmetic, five more instructions; they are what bounds rows of bf16 next to the memory. The K best come without a sort and almost without a second
 // read: the K-th largest of the maxima of 32 groups of threads bounds the K-th largest logit from below, so that only the threads whose maximum reaches the bound
-// look their logits through again, each warp one thread's at a time, and the few logits above it are ranked by counting.
+// have their logits looked through again, and the few logits above it are ranked by counting.
 // Backward: one pass, p from the maximum and the sum; the labels that have a gradient of their own are written once more at the end.
 #include "class_rows.cuh"
 #include "packed_f32.cuh"
@@ -24,9 +24,11 @@ using rows::row_head;
 constexpr int kBack = 256;  // threads of the backward pass
 constexpr int kMaxTop = 32;
 constexpr int kCand = 512;  // logits that are ranked
-// Up to this many best the bound comes from 32 groups of threads (32 shuffles; 12 of 32 are reached by 15 logits on the average), beyond from the threads themselves (a search bit by
-// bit, about a microsecond; 32 of 32 groups would be reached by 130). 1500 rows x 10001 fp32, groups and threads: 8 best 18.1 and 18.8 us, 16 best 23.3 and 22.1, 32 best 56 and 29
-constexpr int kFewTop = 12;
+// Up to this many best the bound comes from 32 groups of threads (32 shuffles; 12 of 32 are reached by 15 logits on the average, 24 by 44), beyond from the threads
+// themselves (a search bit by bit, two microseconds of one warp; 32 of 32 groups would be reached by 130). Few rows wait for the search, many for the instructions.
+// Groups and threads, us: 1500 rows x 10001 fp32, 8 best 16.0 and 17.0, 20 best 20.3 and 19.6, 28 best 27.1 and 21.5; 16 rows x 32000, 20 best 6.1 and 8.1, 24 best 6.5 and 8.1.
+template <int kThreads, int kBatch>
+constexpr int kFewTop = kThreads == 1024 || kBatch == 8 ? 24 : 12;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -94,14 +96,6 @@ __device__ __forceinline__ void in_pairs(const Chunk<false>& u, float least, uin
   for (int i = 0; i < 2; ++i) p[i] = kRaise ? two(max_nan(u.at(2 * i), least), max_nan(u.at(2 * i + 1), least)) : two(u.at(2 * i), u.at(2 * i + 1));
 }
 
-__device__ __forceinline__ void merge(Stat& a, Stat b) {
-  const float nm = fmaxf(a.m, b.m);
-  if (nm > a.m) a.to(nm);
-  if (nm > b.m) b.to(nm);
-  a.s += b.s;
-  a.w += b.w;
-}
-
 // K-th largest of the CTA's whole numbers in shared memory, by one warp, bit by bit (`bits` leading ones may differ)
 template <int kThreads>
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t* key, int k, int bits) {
@@ -139,7 +133,7 @@ struct Best {
   uint64_t cand[kCand];  // rank of the logit, and the label counted from above
   uint64_t last;
   uint32_t bound;
-  int count, found[kThreads / 32];
+  int count, hits, found[kThreads / 32];
 };
 
 // orders logits by rank, then by label from the lowest; below ~0
@@ -155,28 +149,44 @@ __device__ __forceinline__ void consider(Best<kThreads>& b, float x, int label) 
   }
 }
 
-// logits of the threads whose maximum reaches the bound, and those outside the chunks; given up where they are too many
+// logits of the threads whose maximum reaches the bound, and those outside the chunks; given up where they are too many. b.count and b.hits are 0 before. All threads look
+// the chunks of those threads through, two at a time: a warp for its own threads, one after another, waited for the memory at each (1500 x 10001 fp32, 8 best:
+// 18.1 and 15.8 us; 2740 x 1001 fp32, 20 best: 22.9 and 12.4).
 template <int kThreads, bool kBf16>
 __device__ __forceinline__ void collect(Best<kThreads>& b, const Row& r, uint32_t key) {
-  constexpr int kN = Chunk<kBf16>::kN;
+  constexpr int kN = Chunk<kBf16>::kN, kAhead = 2;
   const int lane = threadIdx.x & 31;
-  uint32_t who = __ballot_sync(0xffffffffu, key >= b.bound);
-  while (who && *(volatile int*)&b.count <= kCand) {
-    const int t = __ffs(who) - 1;
-    who &= who - 1;
-    const bool odd = __shfl_sync(0xffffffffu, key, t) == 0xffffffffu;  // (a maximum passes a NaN by)
-    for (int64_t c = r.head + ((threadIdx.x & ~31) + t + (int64_t)kThreads * lane) * kN; c < r.v8; c += 32 * kThreads * kN) {
-      Chunk<kBf16> u;
-      u.load(r.x, r.base + c);
-      if (!odd && rank_of(u.max()) < b.bound) continue;
-#pragma unroll
-      for (int k = 0; k < kN; ++k) consider(b, u.at(k), (int)c + k);
-    }
-  }
+  const uint32_t bound = b.bound, who = __ballot_sync(0xffffffffu, key >= bound);
+  int at = 0;
+  if (lane == 0 && who) at = atomicAdd(&b.hits, __popc(who));
+  at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+  if (key >= bound) b.key[at] = threadIdx.x | (key == 0xffffffffu ? 1u << 31 : 0u);  // (a maximum passes a NaN by)
   const int rest = r.v - (r.v8 - r.head);
   if ((int)threadIdx.x < rest) {
     const int c = (int)threadIdx.x < r.head ? threadIdx.x : threadIdx.x + (r.v8 - r.head);
     consider(b, ld(r.x, r.base + c, kBf16), c);
+  }
+  __syncthreads();
+  const int hits = b.hits, chunks = (r.v8 - r.head + kThreads * kN - 1) / (kThreads * kN);
+  for (int i0 = threadIdx.x; i0 < hits * chunks && *(volatile int*)&b.count <= kCand; i0 += kAhead * kThreads) {
+    Chunk<kBf16> u[kAhead];
+    int c[kAhead];
+    bool odd[kAhead];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int i = i0 + q * kThreads, k = i / hits;
+      const uint32_t t = k < chunks ? b.key[i - k * hits] : 0u;
+      odd[q] = t >> 31;
+      c[q] = r.head + ((int)(t & 0x7fffffffu) + kThreads * k) * kN;
+      if (k < chunks && c[q] < r.v8) u[q].load(r.x, r.base + c[q]);
+      else c[q] = -1;
+    }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      if (c[q] < 0 || (!odd[q] && rank_of(u[q].max()) < bound)) continue;
+#pragma unroll
+      for (int k = 0; k < kN; ++k) consider(b, u[q].at(k), c[q] + k);
+    }
   }
 }
 
@@ -204,7 +214,7 @@ __device__ __forceinline__ uint32_t bound_of_threads(const Best<kThreads>& b, in
 }
 
 // The K best labels of a row in b.cand, in no order; returns how many there are (at least K, all above the K-th and itself among them). b.bound: at most the rank of the
-// K-th largest logit; b.count: 0
+// K-th largest logit; b.count, b.hits: 0
 template <int kThreads, bool kBf16>
 __device__ int select(Best<kThreads>& b, const Row& r, int top, uint32_t key) {
   collect<kThreads, kBf16>(b, r, key);
@@ -214,7 +224,7 @@ __device__ int select(Best<kThreads>& b, const Row& r, int top, uint32_t key) {
   // threads; of those equal to it the lowest labels are taken, in order, a stretch of labels after another.
   __syncthreads();
   b.key[threadIdx.x] = key;
-  if (threadIdx.x == 0) b.count = 0;
+  if (threadIdx.x == 0) b.count = b.hits = 0;
   __syncthreads();
   if (threadIdx.x < 32) {
     const uint32_t bound = bound_of_threads<kThreads, kBf16>(b, top);
@@ -359,7 +369,7 @@ forward_kernel(const Args a) {
   uint32_t key = 0;
   if constexpr (kTop) {
     key = key_of<kThreads, kBf16>(r, st.m, st.s != st.s);
-    if (a.top <= kFewTop) {
+    if (a.top <= kFewTop<kThreads, kBatch>) {
       uint32_t g = key;  // of this thread's group: a warp, or 8 lanes of it
       if (kThreads == 1024) {
         g = __reduce_max_sync(0xffffffffu, g);
@@ -389,17 +399,22 @@ forward_kernel(const Args a) {
   __syncthreads();
   if constexpr (kTop) {
     if (warp == 0) {
-    const uint32_t bound = a.top <= kFewTop ? kth_of_warp(best.group[lane], a.top) : bound_of_threads<kThreads, kBf16>(best, a.top);
+    const uint32_t bound = a.top <= kFewTop<kThreads, kBatch> ? kth_of_warp(best.group[lane], a.top) : bound_of_threads<kThreads, kBf16>(best, a.top);
     if (lane == 0) {
       best.bound = bound;
-      best.count = 0;
+      best.count = best.hits = 0;
     }
     }
   }
+  if (warp == kLast / 32) {  // the warps' sums; one lane after another's would be a microsecond for 32
+    st = lane < kWarps ? Stat{sh_m[lane], sh_s[lane], sh_w[lane]} : Stat{-INFINITY, 0.f, 0.f};
+    const float m = warp_max(st.m);
+    if (m > st.m) st.to(m);
+    st.m = m;
+    st.s = warp_sum(st.s);
+    if (kEntropy) st.w = warp_sum(st.w);
+  }
   if (threadIdx.x == kLast) {
-    st = Stat{sh_m[0], sh_s[0], sh_w[0]};
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) merge(st, Stat{sh_m[w], sh_s[w], sh_w[w]});
     const bool none = st.s == 0.f;  // no label has a probability
     const float log_s = (float)log((double)st.s);
     const float2 norm = none ? make_float2(0.f, -INFINITY) : make_float2(st.m, log_s);
@@ -421,6 +436,7 @@ forward_kernel(const Args a) {
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const uint64_t c = best.cand[i];
       int above = 0;
+#pragma unroll 4
       for (int j = 0; j < n; ++j) above += best.cand[j] > c;
       if (above < a.top) {
         a.top_label[row * a.top + above] = label_of(c);
@@ -559,10 +575,10 @@ RB_EXPORT int rb200_token_log_probs_fwd(const void* x, long long pitch, const vo
   Args a = {};
   a.x = x; a.pitch = pitch; a.target = target; a.target64 = target64; a.v = v; a.top = top; a.lp = lp; a.norm = norm; a.entropy = entropy; a.top_lp = top_lp;
   a.top_label = top_label;
-  // Threads of a row and 16-byte pieces that each has under way. Many rows: 128, 12 rows on an SM, where the latencies of one row's end are hidden best (bf16, us with 128
-  // and 256: 6001 x 32000 without the best 70.1 and 70.8, 8 best 89 and 94; 1500 x 10001 fp32, 8 best 18.1 and 20.8). Fewer do not fill the SMs so: 256 (850 x 32000 fp32,
-  // 32 best: 41.1 and 31.7), and twice the pieces where four rows on an SM are all (500 x 32000: 12.9, with more pieces 9.6; 486 x 128000, 5 best: 49.3 and 36.0). With
-  // two rows on an SM or fewer, 1024 threads for many labels (16 x 32000, 5 best: 8.2 with 256, 6.9; 4 x 128000 fp32, 8 best: 23.0 and 12.5; but 62 x 10001: 3.5 and 4.5).
+  // Threads of a row and 16-byte pieces that each has under way. Many rows: 128, 12 rows on an SM, where the latencies of one row's end are hidden best (us with 128 and 256:
+  // 1500 x 10001 fp32, 8 best 15.9 and 18.3; 6001 x 32000 bf16 70.7 and 69.7, with 8 best 86.9 and 86.7). Fewer do not fill the SMs so: 256 (850 x 32000 fp32, 32 best: 38.5
+  // and 28.1), and twice the pieces where four rows on an SM are all (500 x 32000: 12.9, with more pieces 9.4; 486 x 128000, 5 best: 46.4 and 32.9). With two rows on an SM or
+  // fewer, 1024 threads for many labels (16 x 32000, 5 best: 6.8 with 256, 5.6; 4 x 128000 fp32, 8 best: 21.2 and 10.9; but 183 x 10001, 32 best, with gradient 11.7 and 19.6).
   const int way = rows >= 8 * 148 ? 0 : v < 8192 || rows > 4 * 148 ? 1 : rows > 2 * 148 || v < 16384 ? 2 : 3;
   auto pick = [&](auto threads, auto batch, auto b) {
     constexpr int kT = decltype(threads)::value, kP = decltype(batch)::value;
