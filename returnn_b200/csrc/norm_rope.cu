@@ -10,7 +10,8 @@
 // Rows are read once and written once. A row of D features sits in the next power of two of D / 8 lanes, 8 features a lane, chosen so that both features of a pair
 // are the lane's own: 8 in a row for pairs (2i, 2i + 1), 4 of each half for pairs (i, i + R / 2). The mean is a few shuffles. Head dims, rotated parts and
 // alignments that do not fit this take a warp per row with single elements.
-// What bounds it is the instructions around 16 bytes: each turn of a warp has addresses that only go on by a fixed step.
+// Measured, both passes with the norm: 25000 x 16 heads of 64, bf16, 256 MB, 62.7 us (4.1 TB/s; a copy of as many bytes takes 42), bound by the instructions of a row of 128
+// bytes; 8191 x 40 of 128, fp32, 839 MB, 138.5 us (6.1 TB/s, what the memory gives).
 #include "packed_f32.cuh"
 #include <algorithm>
 #include <cstdlib>
@@ -22,7 +23,7 @@ namespace {
 constexpr int kMaxDim = 256;
 constexpr int kThreads = 256;
 constexpr int kTurnsBf16 = 4, kTurnsF32 = 2, kBackBf16 = 2, kBackF32 = 1;  // rows of a group that are under way at a time, forward and backward
-constexpr int kBackCtas = 4;                                               // of an SM
+constexpr int kCtasBf16 = 4, kCtasF32 = 4, kBackCtasBf16 = 4, kBackCtasF32 = 4;  // of an SM, forward and backward
 
 struct Rows {        // of queries, keys or values
   const void* x;     // input; backward: of the norm (null without one)
@@ -44,8 +45,8 @@ struct Args {
   int64_t n;
   int d, rot, page, pos64, w_bf16, interleaved;
   int tokens;                       // of a CTA's tile
-  int step_tk, step_h;              // of a row of a tile: tokens and heads to the next of its group
-  uint32_t rows_inverse, half_inverse;
+  int split;                        // groups that share a row's tokens where fewer rows are left than groups
+  uint32_t split_inverse, half_inverse;
   float eps, amp, inv_d;
 };
 
@@ -84,16 +85,9 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-struct P4 {  // 8 numbers in pairs
+struct P4 {  // a lane's 8 features in pairs; rotated ones: first the four a of the pairs (a, b), then the four b
   uint64_t v[4];
 };
-__device__ __forceinline__ P4 pairs(const F8& x) { return P4{{two(x.v[0], x.v[1]), two(x.v[2], x.v[3]), two(x.v[4], x.v[5]), two(x.v[6], x.v[7])}}; }
-__device__ __forceinline__ F8 single(const P4& x) {
-  F8 r;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) split(x.v[j], r.v[2 * j], r.v[2 * j + 1]);
-  return r;
-}
 __device__ __forceinline__ P4 scaled(const P4& x, float f) {
   const uint64_t g = two(f, f);
   return P4{{mul2(x.v[0], g), mul2(x.v[1], g), mul2(x.v[2], g), mul2(x.v[3], g)}};
@@ -115,6 +109,14 @@ __device__ __forceinline__ P4 scales_at(const float* p) {
   return P4{{a.x, a.y, b.x, b.y}};
 }
 
+// the same, but from shared memory each time: kept for all rows of a head they are registers that the rows under way need
+__device__ __forceinline__ P4 scales_at(uint32_t p) {
+  P4 r;
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(r.v[0]), "=l"(r.v[1]) : "r"(p) : "memory");
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(r.v[2]), "=l"(r.v[3]) : "r"(p + 16) : "memory");
+  return r;
+}
+
 // A lane's 8 features as they lie in memory: 8 in a row, or twice 4 (kInter false)
 template <typename T, bool kInter>
 struct Raw8;
@@ -129,28 +131,25 @@ struct Raw8<__nv_bfloat16, kInter> {
       u = make_uint4(x.x, x.y, y.x, y.y);
     }
   }
-  __device__ __forceinline__ F8 get() const {
-    F8 r;
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      r.v[2 * i] = __uint_as_float(w[i] << 16);
-      r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-    return r;
+  __device__ __forceinline__ static float lo(uint32_t w) { return __uint_as_float(w << 16); }
+  __device__ __forceinline__ static float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+  __device__ __forceinline__ P4 get() const {
+    if (kInter) return P4{{two(lo(u.x), lo(u.y)), two(lo(u.z), lo(u.w)), two(hi(u.x), hi(u.y)), two(hi(u.z), hi(u.w))}};
+    return P4{{two(lo(u.x), hi(u.x)), two(lo(u.y), hi(u.y)), two(lo(u.z), hi(u.z)), two(lo(u.w), hi(u.w))}};
   }
-  __device__ __forceinline__ static void store(char* p, int gap, const F8& f) {
-    uint32_t w[4];
+  __device__ __forceinline__ static uint32_t word(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ __forceinline__ static void store(char* p, int gap, const P4& x) {
+    float f[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f.v[2 * i], f.v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
+    for (int j = 0; j < 4; ++j) split(x.v[j], f[2 * j], f[2 * j + 1]);
     if (kInter) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(p) = make_uint4(word(f[0], f[4]), word(f[1], f[5]), word(f[2], f[6]), word(f[3], f[7]));
     } else {
-      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-      *reinterpret_cast<uint2*>(p + gap) = make_uint2(w[2], w[3]);
+      *reinterpret_cast<uint2*>(p) = make_uint2(word(f[0], f[1]), word(f[2], f[3]));
+      *reinterpret_cast<uint2*>(p + gap) = make_uint2(word(f[4], f[5]), word(f[6], f[7]));
     }
   }
 };
@@ -161,10 +160,21 @@ struct Raw8<float, kInter> {
     a = *reinterpret_cast<const float4*>(p);
     b = *reinterpret_cast<const float4*>(p + gap);
   }
-  __device__ __forceinline__ F8 get() const { return F8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}}; }
-  __device__ __forceinline__ static void store(char* p, int gap, const F8& f) {
-    *reinterpret_cast<float4*>(p) = make_float4(f.v[0], f.v[1], f.v[2], f.v[3]);
-    *reinterpret_cast<float4*>(p + gap) = make_float4(f.v[4], f.v[5], f.v[6], f.v[7]);
+  __device__ __forceinline__ P4 get() const {
+    if (kInter) return P4{{two(a.x, a.z), two(b.x, b.z), two(a.y, a.w), two(b.y, b.w)}};
+    return P4{{two(a.x, a.y), two(a.z, a.w), two(b.x, b.y), two(b.z, b.w)}};
+  }
+  __device__ __forceinline__ static void store(char* p, int gap, const P4& x) {
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split(x.v[j], f[2 * j], f[2 * j + 1]);
+    if (kInter) {
+      *reinterpret_cast<float4*>(p) = make_float4(f[0], f[4], f[1], f[5]);
+      *reinterpret_cast<float4*>(p + gap) = make_float4(f[2], f[6], f[3], f[7]);
+    } else {
+      *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+      *reinterpret_cast<float4*>(p + gap) = make_float4(f[4], f[5], f[6], f[7]);
+    }
   }
 };
 
@@ -190,63 +200,68 @@ __device__ __forceinline__ Lane lane_of(const Args& a) {
   return l;
 }
 
-// the four pairs of a lane turned (sign -1: back)
-template <bool kInter>
-__device__ __forceinline__ void rotate4(F8& x, const float2* table, const Lane& l, float sign) {
-  if (!l.turned) return;
-  const float4* t = reinterpret_cast<const float4*>(table + l.sub * 4);
-  const float4 t0 = t[0], t1 = t[1];
-  const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y * sign, t0.w * sign, t1.y * sign, t1.w * sign};
+// the four pairs of a lane turned; t: their four cosines and four sines
+__device__ __forceinline__ void rotate4(P4& x, const float* t) {
+  const P4 cs = scales_at(t);
+  const uint64_t minus = two(-1.f, -1.f);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float &p = x.v[kInter ? 2 * j : j], &q = x.v[kInter ? 2 * j + 1 : 4 + j];
-    const float u = p * c[j] - q * s[j];
-    q = p * s[j] + q * c[j];
-    p = u;
+  for (int j = 0; j < 2; ++j) {
+    const uint64_t a = x.v[j], b = x.v[2 + j], c = cs.v[j], s = cs.v[2 + j];
+    x.v[j] = fma2(a, c, mul2(mul2(b, minus), s));
+    x.v[2 + j] = fma2(a, s, mul2(b, c));
   }
 }
 
-// A CTA has the rows (token, head) of a few tokens, queries' heads before keys' and values', a row per group of kLanes lanes and turn. Rows go on by whole steps, so that token
-// and head cost no division; offsets within a tile of tokens are 32 bits wide (see fits).
-struct Walk {
-  int tk, h;
-  __device__ __forceinline__ Walk(int start, uint32_t inverse, int of) {  // inverse: 2^32 / of, rounded up; start below 2^16
-    tk = of == 1 ? start : (int)__umulhi((uint32_t)start, inverse);
-    h = start - tk * of;
-  }
-  __device__ __forceinline__ void go(const Args& a, int of) {
-    tk += a.step_tk;
-    h += a.step_h;
-    if (h >= of) {
-      h -= of;
-      ++tk;
-    }
+// A CTA has the rows (token, head) of a few tokens. A group of kLanes lanes keeps to one head at a time, of the queries' or then the keys' or the values', and goes through the
+// tokens: scale, strides and addresses stay, a row costs no selection. Where fewer heads are left than groups, `split` groups share the tokens of a head. (With the rows of a
+// tile counted through, token after token, half of the instructions were addresses and choices: 25000 tokens x 16
+// heads of 64, bf16, both passes, 70.4 us, by heads 65.0.)
+struct Turn {
+  int tk, row, split;  // first token of this group, its head, tokens to the next
+  bool mine;
+  __device__ __forceinline__ Turn(const Args& a, int row0, int rows, int group, int groups) {
+    const bool whole = rows - row0 >= groups;
+    const int left = whole ? groups : rows - row0;
+    tk = whole ? 0 : left == 1 ? group : (int)__umulhi((uint32_t)group, a.split_inverse);
+    row = row0 + group - tk * left;
+    split = whole ? 1 : a.split;
+    mine = tk < split;
   }
 };
 
-// shared memory: the scales of queries and keys in fp32 in the lanes' order, [2][kLanes * 8]; then the angles of the tile's tokens, [tokens][R / 2]
+// feature that a lane has in place `in` of its 8
+template <bool kInter>
+__device__ __forceinline__ int feature_at(const Args& a, int sub, int in) {
+  if (kInter) return sub * 8 + (in < 4 ? 2 * in : 2 * in - 7);
+  if (sub * 8 < a.rot) return in < 4 ? sub * 4 + in : (a.rot >> 1) + sub * 4 + in - 4;
+  return sub * 8 + in;
+}
+// shared memory: the scales of queries and keys in fp32 in the lanes' order, [2][kLanes * 8]; then the cosines and sines of the tile's tokens, [tokens][R / 8][2][4]
 template <bool kInter, int kLanes>
 __device__ __forceinline__ void fill_scales(const Args& a, float* scales) {
   if (!a.r[0].w) return;
   for (int i = threadIdx.x; i < 2 * kLanes * 8; i += kThreads) {
-    const int e = i % (kLanes * 8), sub = e >> 3, in = e & 7;
-    int at = e;
-    if (!kInter && sub * 8 < a.rot) at = in < 4 ? sub * 4 + in : (a.rot >> 1) + sub * 4 + in - 4;
-    scales[i] = e < a.d ? weight_at(i < kLanes * 8 ? a.r[0].w : a.r[1].w, at, a.w_bf16) : 0.f;
+    const int e = i % (kLanes * 8);
+    scales[i] = e < a.d ? weight_at(i < kLanes * 8 ? a.r[0].w : a.r[1].w, feature_at<kInter>(a, e >> 3, e & 7), a.w_bf16) : 0.f;
   }
 }
-__device__ __forceinline__ void fill_table(const Args& a, float2* table, int64_t t0, int nt) {
+__device__ __forceinline__ void fill_table(const Args& a, float* table, int64_t t0, int nt, float sign) {
   const int half = a.rot >> 1;
   if (!half) return;
-  const Walk w(threadIdx.x, a.half_inverse, half);  // (an angle per thread: see tile_of)
-  if (w.tk < nt) table[threadIdx.x] = turn_of(a, position_of(a, t0 + w.tk), turns_of(a, w.h));
+  for (int i = threadIdx.x; i < nt * half; i += kThreads) {
+    const int tk = (int)__umulhi(i, a.half_inverse), pair = i - tk * half;  // (half is 4 at least)
+    const float2 t = turn_of(a, position_of(a, t0 + tk), turns_of(a, pair));
+    float* to = table + tk * a.rot + (pair >> 2) * 8 + (pair & 3);
+    to[0] = t.x;
+    to[4] = t.y * sign;
+  }
 }
 
 template <typename T, bool kInter, bool kCache, int kLanes>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? kCtasBf16 : kCtasF32)
 forward_kernel(const Args a) {
   extern __shared__ __align__(16) float smem[];
-  float2* table = reinterpret_cast<float2*>(smem + 2 * kLanes * 8);
+  float* table = smem + 2 * kLanes * 8;
   rb_pdl_wait();
   rb_pdl_launch();
   constexpr int kTurns = sizeof(T) == 2 ? kTurnsBf16 : kTurnsF32, kSize = sizeof(T), kGroups = kThreads / kLanes;
@@ -254,60 +269,53 @@ forward_kernel(const Args a) {
   const Lane l = lane_of<kInter, kLanes>(a);
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
   const int nt = (int)min((int64_t)a.tokens, a.n - t0);
-  const int hq = a.r[0].heads, hk = a.r[1].heads, rows = hq + hk + (kCache ? hk : 0), half = a.rot >> 1;
+  const int hq = a.r[0].heads, hk = a.r[1].heads, rows = hq + hk + (kCache ? hk : 0), groups = gridDim.y * kGroups;
   const bool norm = a.r[0].w != nullptr;
   const int gap = l.gap * kSize;
-  const char* in_q = reinterpret_cast<const char*>(a.r[0].x) + (t0 * a.r[0].tok + l.at) * kSize;
-  const char* in_k = reinterpret_cast<const char*>(a.r[1].x) + (t0 * a.r[1].tok + l.at) * kSize;
-  const char* in_v = kCache ? reinterpret_cast<const char*>(a.r[2].x) + (t0 * a.r[2].tok + l.at) * kSize : nullptr;
-  char* out_q = reinterpret_cast<char*>(a.r[0].out) + (t0 * hq * a.d + l.at) * kSize;
-  char* out_k = kCache ? nullptr : reinterpret_cast<char*>(a.r[1].out) + (t0 * hk * a.d + l.at) * kSize;
-  const int total = nt * rows, step = gridDim.y * kGroups;
-  Walk fetch(blockIdx.y * kGroups + threadIdx.x / kLanes, a.rows_inverse, rows), use = fetch;
   bool ready = false;
-  for (int r = blockIdx.y * kGroups; r < total; r += kTurns * step) {
-    Raw raw[kTurns] = {};
+  for (int row0 = 0; row0 < rows; row0 += groups) {
+    const Turn turn(a, row0, rows, blockIdx.y * kGroups + threadIdx.x / kLanes, groups);
+    const bool is_q = turn.row < hq, is_v = kCache && turn.row >= hq + hk, mine = turn.mine && l.real;
+    const Rows& w = a.r[is_q ? 0 : is_v ? 2 : 1];
+    const int h = is_q ? turn.row : is_v ? turn.row - hq - hk : turn.row - hq;
+    const char* from = reinterpret_cast<const char*>(w.x) + ((t0 + turn.tk) * w.tok + h * w.head + l.at) * kSize;
+    const int step = turn.split * (int)w.tok * kSize, out_step = turn.split * w.heads * a.d * kSize;
+    char* to = reinterpret_cast<char*>(w.out) + (kCache && !is_q ? h * w.page_head + l.at : ((t0 + turn.tk) * w.heads + h) * a.d + l.at) * kSize;
+    P4 scales;
+    for (int t = 0; t < nt; t += kTurns * turn.split) {
+      Raw raw[kTurns] = {};
 #pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
-      if (fetch.tk < nt && l.real) {
-        const bool is_q = fetch.h < hq, is_v = kCache && fetch.h >= hq + hk;
-        const int tok = (int)(is_q ? a.r[0].tok : is_v ? a.r[2].tok : a.r[1].tok), head = (int)(is_q ? a.r[0].head : is_v ? a.r[2].head : a.r[1].head);
-        const int h = is_q ? fetch.h : is_v ? fetch.h - hq - hk : fetch.h - hq;
-        raw[u].load((is_q ? in_q : is_v ? in_v : in_k) + (fetch.tk * tok + h * head) * kSize, gap);
+      for (int u = 0; u < kTurns; ++u) {
+        if (mine && turn.tk + t + u * turn.split < nt) raw[u].load(from, gap);
+        from += step;
       }
-      fetch.go(a, rows);
-    }
-    if (!ready) {  // while the first rows are under way
-      fill_scales<kInter, kLanes>(a, smem);
-      fill_table(a, table, t0, nt);
-      __syncthreads();
-      ready = true;
-    }
+      if (!ready) {  // while the first rows are under way
+        fill_scales<kInter, kLanes>(a, smem);
+        fill_table(a, table, t0, nt, 1.f);
+        __syncthreads();
+        ready = true;
+      }
+      if (norm && t == 0) scales = scales_at(smem + (is_q ? 0 : kLanes * 8) + l.sub * 8);
 #pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
-      if (r + u * step < total) {
-        const bool live = use.tk < nt && l.real, is_q = use.h < hq, is_v = kCache && use.h >= hq + hk;
-        F8 y = raw[u].get();
-        if (norm) {
-          const P4 x = pairs(y);
-          const float inv = rsqrtf(group_sum(dot_of(x, x), kLanes) * a.inv_d + a.eps);
-          if (!is_v) y = single(product(scaled(x, inv), scales_at(smem + (is_q ? 0 : kLanes * 8) + l.sub * 8)));
-        }
-        if (live) {
-          if (!is_v) rotate4<kInter>(y, table + use.tk * half, l, 1.f);
-          char* out;
-          if (is_q) {
-            out = out_q + (use.tk * hq + use.h) * (a.d * kSize);
-          } else if (!kCache) {
-            out = out_k + (use.tk * hk + use.h - hq) * (a.d * kSize);
-          } else {
-            const Rows& k = is_v ? a.r[2] : a.r[1];
-            const int64_t at = cache_at(a, k, t0 + use.tk);
-            out = at < 0 ? nullptr : reinterpret_cast<char*>(k.out) + (at + (is_v ? use.h - hq - hk : use.h - hq) * k.page_head + l.at) * kSize;
+      for (int u = 0; u < kTurns; ++u) {
+        if (t + u * turn.split < nt) {
+          const int tk = turn.tk + t + u * turn.split;
+          P4 y = raw[u].get();
+          if (norm) {
+            const float inv = rsqrtf(group_sum(dot_of(y, y), kLanes) * a.inv_d + a.eps);
+            if (!is_v) y = product(scaled(y, inv), scales);
           }
-          if (!kCache || out) Raw::store(out, gap, y);
+          if (mine && tk < nt) {
+            if (!is_v && l.turned) rotate4(y, table + tk * a.rot + l.sub * 8);
+            if (!kCache || is_q) {
+              Raw::store(to, gap, y);
+            } else {
+              const int64_t at = cache_at(a, w, t0 + tk);
+              if (at >= 0) Raw::store(to + at * kSize, gap, y);
+            }
+          }
+          if (!kCache || is_q) to += out_step;
         }
-        use.go(a, rows);
       }
     }
   }
@@ -315,97 +323,97 @@ forward_kernel(const Args a) {
 
 // kNorm: x is read again and the weights have gradients (sums per CTA, added up in order by the kernel below)
 template <typename T, bool kInter, bool kNorm, int kLanes>
-__global__ void __launch_bounds__(kThreads, kBackCtas)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? kBackCtasBf16 : kBackCtasF32)
 backward_kernel(const Args a) {
   extern __shared__ __align__(16) float smem[];
-  float2* table = reinterpret_cast<float2*>(smem + 2 * kLanes * 8);
+  float* table = smem + 2 * kLanes * 8;
   rb_pdl_wait();
   rb_pdl_launch();
   constexpr int kTurns = sizeof(T) == 2 ? kBackBf16 : kBackF32, kSize = sizeof(T), kGroups = kThreads / kLanes;
   using Raw = Raw8<T, kInter>;
   const Lane l = lane_of<kInter, kLanes>(a);
-  const int hq = a.r[0].heads, hk = a.r[1].heads, rows = hq + hk, half = a.rot >> 1;
+  const int hq = a.r[0].heads, hk = a.r[1].heads, rows = hq + hk;
   const int gap = l.gap * kSize;
-  P4 gq = {}, gk = {};
+  // sums of the scales' gradients: this thread's 8 of queries and of keys, touched once per head and tile
+  float* sums = smem + 2 * kLanes * 8 + a.tokens * a.rot;
+  ulonglong2* mine_q = reinterpret_cast<ulonglong2*>(sums) + threadIdx.x * 2;  // [2][groups][lanes * 8]
+  ulonglong2* mine_k = mine_q + kThreads * 2;
+  if (kNorm) mine_q[0] = mine_q[1] = mine_k[0] = mine_k[1] = make_ulonglong2(0, 0);
   bool have_scales = false;
   for (int64_t t0 = (int64_t)blockIdx.x * a.tokens; t0 < a.n; t0 += (int64_t)gridDim.x * a.tokens) {
     const int nt = (int)min((int64_t)a.tokens, a.n - t0);
-    const char* dz_q = reinterpret_cast<const char*>(a.r[0].dz) + (t0 * a.r[0].dz_tok + l.at) * kSize;
-    const char* dz_k = reinterpret_cast<const char*>(a.r[1].dz) + (t0 * a.r[1].dz_tok + l.at) * kSize;
-    const char* in_q = reinterpret_cast<const char*>(a.r[0].x) + (t0 * a.r[0].tok + l.at) * kSize;
-    const char* in_k = reinterpret_cast<const char*>(a.r[1].x) + (t0 * a.r[1].tok + l.at) * kSize;
-    char* out_q = reinterpret_cast<char*>(a.r[0].out) + (t0 * hq * a.d + l.at) * kSize;
-    char* out_k = reinterpret_cast<char*>(a.r[1].out) + (t0 * hk * a.d + l.at) * kSize;
-    const int total = nt * rows;
-    Walk fetch(threadIdx.x / kLanes, a.rows_inverse, rows), use = fetch;
-    for (int r = 0; r < total; r += kTurns * kGroups) {
-      Raw raw_g[kTurns] = {}, raw_x[kNorm ? kTurns : 1] = {};
+    for (int row0 = 0; row0 < rows; row0 += gridDim.y * kGroups) {
+      const Turn turn(a, row0, rows, blockIdx.y * kGroups + threadIdx.x / kLanes, gridDim.y * kGroups);
+      const bool is_q = turn.row < hq, mine = turn.mine && l.real;
+      const Rows& w = a.r[is_q ? 0 : 1];
+      const int h = is_q ? turn.row : turn.row - hq;
+      const char* from_z = reinterpret_cast<const char*>(w.dz) + ((t0 + turn.tk) * w.dz_tok + h * w.dz_head + l.at) * kSize;
+      const char* from_x = reinterpret_cast<const char*>(w.x) + ((t0 + turn.tk) * w.tok + h * w.head + l.at) * kSize;
+      const int step_z = turn.split * (int)w.dz_tok * kSize, step_x = turn.split * (int)w.tok * kSize, out_step = turn.split * w.heads * a.d * kSize;
+      char* to = reinterpret_cast<char*>(w.out) + (((t0 + turn.tk) * w.heads + h) * a.d + l.at) * kSize;
+      P4 sum = {};
+      const uint32_t at_scales = (uint32_t)__cvta_generic_to_shared(smem + (is_q ? 0 : kLanes * 8) + l.sub * 8);
+      for (int t = 0; t < nt; t += kTurns * turn.split) {
+        Raw raw_z[kTurns] = {}, raw_x[kNorm ? kTurns : 1] = {};
 #pragma unroll
-      for (int u = 0; u < kTurns; ++u) {
-        if (fetch.tk < nt && l.real) {
-          const bool is_q = fetch.h < hq;
-          const int h = is_q ? fetch.h : fetch.h - hq;
-          raw_g[u].load((is_q ? dz_q : dz_k) + (fetch.tk * (int)(is_q ? a.r[0].dz_tok : a.r[1].dz_tok) + h * (int)(is_q ? a.r[0].dz_head : a.r[1].dz_head)) * kSize, gap);
-          if (kNorm) raw_x[u].load((is_q ? in_q : in_k) + (fetch.tk * (int)(is_q ? a.r[0].tok : a.r[1].tok) + h * (int)(is_q ? a.r[0].head : a.r[1].head)) * kSize, gap);
-        }
-        fetch.go(a, rows);
-      }
-      if (r == 0) {
-        __syncthreads();  // (the table of the tokens before has been read)
-        if (!have_scales) fill_scales<kInter, kLanes>(a, smem);
-        have_scales = true;
-        fill_table(a, table, t0, nt);
-        __syncthreads();
-      }
-#pragma unroll
-      for (int u = 0; u < kTurns; ++u) {
-        if (r + u * kGroups < total) {
-          const bool live = use.tk < nt && l.real, is_q = use.h < hq;
-          F8 g = raw_g[u].get();
-          if (live) rotate4<kInter>(g, table + use.tk * half, l, -1.f);
-          if (kNorm) {
-            const P4 x = pairs(raw_x[u].get());
-            const float inv = rsqrtf(group_sum(dot_of(x, x), kLanes) * a.inv_d + a.eps);
-            const P4 v = scaled(x, inv), dy = pairs(g);
-            const uint64_t yes = two(is_q ? 1.f : 0.f, is_q ? 1.f : 0.f), no = two(is_q ? 0.f : 1.f, is_q ? 0.f : 1.f);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint64_t e = mul2(dy.v[j], v.v[j]);  // (zeros in lanes and groups without a row)
-              gq.v[j] = fma2(e, yes, gq.v[j]);
-              gk.v[j] = fma2(e, no, gk.v[j]);
-            }
-            const P4 w = product(dy, scales_at(smem + (is_q ? 0 : kLanes * 8) + l.sub * 8));
-            const float dot = -group_sum(dot_of(w, v), kLanes) * a.inv_d * inv;
-            const uint64_t by = two(inv, inv), off = two(dot, dot);
-            P4 r;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r.v[j] = fma2(v.v[j], off, mul2(w.v[j], by));
-            g = single(r);
+        for (int u = 0; u < kTurns; ++u) {
+          if (mine && turn.tk + t + u * turn.split < nt) {
+            raw_z[u].load(from_z, gap);
+            if (kNorm) raw_x[u].load(from_x, gap);
           }
-          if (live) Raw::store(is_q ? out_q + (use.tk * hq + use.h) * (a.d * kSize) : out_k + (use.tk * hk + use.h - hq) * (a.d * kSize), gap, g);
-          use.go(a, rows);
+          from_z += step_z;
+          if (kNorm) from_x += step_x;
         }
+        if (row0 == 0 && t == 0) {
+          __syncthreads();  // (the table of the tokens before has been read)
+          if (!have_scales) fill_scales<kInter, kLanes>(a, smem);
+          have_scales = true;
+          fill_table(a, table, t0, nt, -1.f);
+          __syncthreads();
+        }
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u) {
+          if (t + u * turn.split < nt) {
+            const int tk = turn.tk + t + u * turn.split;
+            const bool live = mine && tk < nt;
+            P4 g = raw_z[u].get();
+            if (live && l.turned) rotate4(g, table + tk * a.rot + l.sub * 8);
+            if (kNorm) {
+              const P4 x = raw_x[u].get();
+              const float inv = rsqrtf(group_sum(dot_of(x, x), kLanes) * a.inv_d + a.eps);
+              const P4 v = scaled(x, inv);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sum.v[j] = fma2(g.v[j], v.v[j], sum.v[j]);  // (zeros in lanes and groups without a row)
+              const P4 y = product(g, scales_at(at_scales));
+              const float dot = -group_sum(dot_of(y, v), kLanes) * a.inv_d * inv;
+              const uint64_t by = two(inv, inv), off = two(dot, dot);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) g.v[j] = fma2(v.v[j], off, mul2(y.v[j], by));
+            }
+            if (live) Raw::store(to, gap, g);
+            to += out_step;
+          }
+        }
+      }
+      if (kNorm) {
+        ulonglong2* to_sum = is_q ? mine_q : mine_k;
+        const ulonglong2 s0 = to_sum[0], s1 = to_sum[1];
+        to_sum[0] = make_ulonglong2(add2(s0.x, sum.v[0]), add2(s0.y, sum.v[1]));
+        to_sum[1] = make_ulonglong2(add2(s1.x, sum.v[2]), add2(s1.y, sum.v[3]));
       }
     }
   }
   if (kNorm) {
-    float* sums = smem;  // [groups][2][lanes * 8] in the lanes' order; at least as large as this (see the launch)
-    __syncthreads();
-    float* mine = sums + threadIdx.x / kLanes * 2 * kLanes * 8;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      reinterpret_cast<uint64_t*>(mine + l.sub * 8)[j] = gq.v[j];
-      reinterpret_cast<uint64_t*>(mine + kLanes * 8 + l.sub * 8)[j] = gk.v[j];
-    }
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * a.d; i += kThreads) {
       const int e = i < a.d ? i : i - a.d, half = a.rot >> 1;
       int at = e;  // where the lanes have feature e
-      if (!kInter && e < a.rot) at = e < half ? (e >> 2) * 8 + (e & 3) : ((e - half) >> 2) * 8 + 4 + ((e - half) & 3);
-      if (i >= a.d) at += kLanes * 8;
+      if (kInter) at = (e & ~7) + (e & 1) * 4 + ((e & 7) >> 1);
+      else if (e < a.rot) at = e < half ? (e >> 2) * 8 + (e & 3) : ((e - half) >> 2) * 8 + 4 + ((e - half) & 3);
+      if (i >= a.d) at += kThreads * 8;
       float s = 0.f;
-      for (int g = 0; g < kThreads / kLanes; ++g) s += sums[g * 2 * kLanes * 8 + at];
-      a.part[(int64_t)blockIdx.x * 2 * a.d + i] = s;
+      for (int g = 0; g < kThreads / kLanes; ++g) s += sums[g * kLanes * 8 + at];
+      a.part[(int64_t)(blockIdx.y * gridDim.x + blockIdx.x) * 2 * a.d + i] = s;
     }
   }
 }
@@ -609,7 +617,7 @@ int bad_shape(const Args& a) {
   return 1;
 }
 
-// 8 features a lane, whole pairs, vector accesses (16 bytes; pairs (i, i + R / 2) in bf16: 8), tiles below 2^31 bytes
+// 8 features a lane, whole pairs, vector accesses (16 bytes; pairs (i, i + R / 2) in bf16: 8)
 bool fits(const Args& a, int bf16, bool backward, bool cache) {
   const int bytes = bf16 && !a.interleaved ? 8 : 16, unit = bytes / (bf16 ? 2 : 4);
   if (a.d % 8 || a.rot % 8) return false;
@@ -620,28 +628,45 @@ bool fits(const Args& a, int bf16, bool backward, bool cache) {
     if (!backward || a.r[0].w) ok = ok && aligned(r.x, {r.tok, r.head}, unit, bytes);
     if (backward) ok = ok && aligned(r.dz, {r.dz_tok, r.dz_head}, unit, bytes);
     if (cache && i) ok = ok && aligned(r.out, {r.page, r.page_head, r.page_tok}, unit, bytes);
-    // offsets within a tile of up to 256 tokens
-    const int64_t widest = std::max({std::abs(r.head), std::abs(r.dz_head), (int64_t)a.d}) * r.heads + std::max(std::abs(r.tok), std::abs(r.dz_tok)) * 256;
-    ok = ok && widest * 4 < (int64_t)1 << 31 && (int64_t)a.d * r.heads * 256 * 4 < (int64_t)1 << 31;
+    // steps of up to 256 tokens in 32 bits, group numbers in 16
+    ok = ok && std::max({std::abs(r.tok), std::abs(r.dz_tok), (int64_t)a.d * r.heads}) * 256 * 4 < (int64_t)1 << 31 && r.heads < 16384;
   }
   return ok;
 }
 
-// A tile is as many tokens as fill the table with an angle per thread; fewer where that leaves SMs without any
-void tile_of(Args& a) {
+// A tile is as many tokens as fill the table with an angle per thread; fewer where that leaves SMs without any. A CTA of the backward pass has one tile after another, each with a
+// beginning that costs about as much as two rows of a group: tiles are up to four times as large where the turns that all tiles take are the shorter for it (8191 tokens x 40
+// rows of 128, bf16, both passes: 103.6 us with 4 tokens, 97.1 with 16; 20000 x 24 of 64 take 8, 5 turns of which are shorter than 3 of 16). Where all tiles are on the SMs at once, their heads are shared by
+// as many CTAs as it takes for every group to have one head (returned): all rows are then asked for at the beginning.
+int tile_of(Args& a, int rows, int groups, int ctas, bool backward) {
+  const int need = std::max(1, (rows + groups - 1) / groups);
+  auto tiles = [&]() { return (a.n + a.tokens - 1) / a.tokens; };
   a.tokens = a.rot ? std::max(1, kThreads / (a.rot / 2)) : 8;
-  while (a.tokens > 1 && (a.n + a.tokens - 1) / a.tokens < 2 * 148) a.tokens /= 2;
-}
-// rows of a tile, `step` groups at a time
-void walk_of(Args& a, int rows, int step) {
-  a.step_tk = step / rows;
-  a.step_h = step % rows;
-  a.rows_inverse = rows > 1 ? (uint32_t)(((1ull << 32) + rows - 1) / rows) : 0u;
-  a.half_inverse = a.rot > 2 ? (uint32_t)(((1ull << 32) + a.rot / 2 - 1) / (a.rot / 2)) : 0u;
+  if (backward) {
+    const int least = a.tokens;
+    auto turns = [&]() { return ((tiles() + ctas * 148 - 1) / (ctas * 148)) * (a.tokens * (int64_t)rows + 2 * groups); };
+    int best = least;
+    int64_t cost = turns();
+    for (int more = 2; more <= 4; more *= 2) {
+      a.tokens = least * more;
+      if (tiles() < 2 * 148 || turns() >= cost) continue;
+      best = a.tokens;
+      cost = turns();
+    }
+    a.tokens = best;
+  }
+  while (a.tokens > 1 && tiles() * need < 2 * 148) a.tokens /= 2;
+  const int shared_by = tiles() * need <= ctas * 148 ? need : 1;
+  while (a.tokens > 1 && tiles() * shared_by < 2 * 148) a.tokens /= 2;
+  const int left = rows % (groups * shared_by);
+  a.split = left ? groups * shared_by / left : 1;
+  a.split_inverse = left > 1 ? (uint32_t)(((1ull << 32) + left - 1) / left) : 0u;
+  a.half_inverse = a.rot ? (uint32_t)(((1ull << 32) + a.rot / 2 - 1) / (a.rot / 2)) : 0u;
+  return shared_by;
 }
 size_t smem_of(const Args& a) { return (size_t)lanes_of(a.d) * 16 * sizeof(float) + (size_t)a.tokens * (a.rot / 2) * sizeof(float2); }
 
-constexpr int kParts = 148 * kBackCtas;
+constexpr int kParts = 148 * std::max(kBackCtasBf16, kBackCtasF32);
 
 int forward(Args& a, int bf16, bool cache, cudaStream_t stream) {
   if (bad_shape(a)) return RB_ERR_UNSUPPORTED;
@@ -649,12 +674,8 @@ int forward(Args& a, int bf16, bool cache, cudaStream_t stream) {
   if (a.n <= 0 || rows == 0) return RB_OK;
   a.inv_d = 1.f / a.d;
   if (fits(a, bf16, false, cache)) {
-    tile_of(a);
-    const int groups = kThreads / lanes_of(a.d);
+    const int gy = tile_of(a, rows, kThreads / lanes_of(a.d), bf16 ? kCtasBf16 : kCtasF32, false);
     const int64_t gx = (a.n + a.tokens - 1) / a.tokens;
-    int gy = 1;  // where tokens are few their rows are shared by several CTAs
-    while (gx * gy < 148 && gy * groups < a.tokens * rows) gy *= 2;
-    walk_of(a, rows, gy * groups);
     if (gx > 0x7fffffff) {
       rb_set_error("norm_rope: %lld tokens", (long long)a.n);
       return RB_ERR_UNSUPPORTED;
@@ -744,10 +765,11 @@ RB_EXPORT int rb200_norm_rope_bwd(const void* dq, const void* dk, const void* q,
   if (!norm && (n <= 0 || rows == 0)) return RB_OK;
   a.inv_d = 1.f / d;
   int64_t grid;  // (without any row one CTA leaves sums of zero)
+  int gy = 1;
   if (fits(a, bf16, true, false)) {
-    tile_of(a);
-    walk_of(a, std::max(rows, 1), kThreads / lanes_of(d));
-    grid = std::max<int64_t>(1, std::min<int64_t>((n + a.tokens - 1) / a.tokens, kParts));
+    const int ctas = bf16 ? kBackCtasBf16 : kBackCtasF32;
+    gy = tile_of(a, rows, kThreads / lanes_of(d), ctas, true);
+    grid = std::max<int64_t>(1, std::min<int64_t>((n + a.tokens - 1) / a.tokens, 148 * ctas / gy));
     const size_t sums = norm ? (size_t)kThreads * 2 * 8 * sizeof(float) : 0;
     auto pick = [&](auto t) {
       return with_lanes(d, [&](auto l) {
@@ -758,12 +780,12 @@ RB_EXPORT int rb200_norm_rope_bwd(const void* dq, const void* dk, const void* q,
       });
     };
     auto kernel = bf16 ? pick(__nv_bfloat16()) : pick(float());
-    rb_launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), std::max(smem_of(a), sums), stream, a);
+    rb_launch_pdl(kernel, dim3((unsigned)grid, (unsigned)gy), dim3(kThreads), smem_of(a) + sums, stream, a);
   } else {
     grid = std::max<int64_t>(1, std::min<int64_t>((n * rows + kThreads / 32 - 1) / (kThreads / 32), kParts));
     auto kernel = bf16 ? backward_any_kernel<__nv_bfloat16> : backward_any_kernel<float>;
     rb_launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
   }
-  if (norm) rb_launch_pdl(weight_sum_kernel, dim3((2 * d + 31) / 32), dim3(kSumWarps * 32), 0, stream, (const float*)part, (int)grid, d, dwq, dwk, w_bf16);
+  if (norm) rb_launch_pdl(weight_sum_kernel, dim3((2 * d + 31) / 32), dim3(kSumWarps * 32), 0, stream, (const float*)part, (int)grid * gy, d, dwq, dwk, w_bf16);
   return rb_check_launch("norm_rope_bwd");
 }
