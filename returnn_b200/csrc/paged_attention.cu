@@ -17,9 +17,11 @@
 // larger tensor-memory instructions have nothing to win (64 rows at least, keys would pass through descriptors) and the sixteen rows here are only half used:
 // rows 0..7 are 8 query heads with the weights rounded to bf16, rows 8..15 the same heads with what the rounding lost. Their sum weighs the
 // values with 16 bits of mantissa at no further instruction; weights of 8 bits would add an error as large as the rounding of the result.
-// fp32: products by fused multiply-adds.
+// fp32: products by fused multiply-adds, a kernel for 1, 2, 4 and 8 heads of a unit (14 requests, 56340 tokens, D 128, 4 on each of 8 key heads: 89 us; with one kernel and the heads
+// counted at run time 169).
 // Measured (D 128, 4 query heads on each of 8 key heads, bf16): 64 requests of 122637 tokens together, 502 MB, 85 us (5.9 TB/s); two of 76484 and 131072, 850 MB, 133 us
-// (6.4 TB/s). Small calls are the launches and the chain of length, page, token, product and join: one request of 1000 tokens, fp32, D 64, 10.5 us.
+// (6.4 TB/s). Small calls are the launches and the chain of length, page, token, product and join: one request of 1000 tokens, fp32, D 64, 9.1 us.
+#include "packed_f32.cuh"
 #include "tcgen05.cuh"
 #include <algorithm>
 
@@ -46,17 +48,18 @@ struct Args {
   float scale_log2;
 };
 
-template <typename T, int DP>
+// H: query heads that a multiplying warp computes (bf16: the 8 of a product)
+template <typename T, int DP, int H>
 struct Shape {
   static constexpr bool kBf16 = sizeof(T) == 2;
   static constexpr int kRowBytes = DP * (int)sizeof(T);
-  static constexpr int kRows = kRowBytes <= 512 ? 16 : 8;  // tokens of a part
+  static constexpr int kRows = kRowBytes <= (kBf16 ? 512 : 256) ? 16 : 8;  // tokens of a part
   static constexpr int kPart = kRows * kRowBytes;          // blocks of kRows rows of 128 bytes, 16-byte pieces swizzled by the row
-  static constexpr int kWarps = kRowBytes <= 256 ? 8 : 4;
+  static constexpr int kWarps = kRows * kRowBytes <= 4096 ? 8 : 4;
   static constexpr int kStage = 2 * kWarps * kPart;  // keys, values
   static constexpr int kPitch = DP + 8;              // floats of a head where the warps meet (no bank conflicts)
-  static constexpr int kMeet = 8 * kPitch + 16;      // of a warp: outputs, maxima, sums; fp32: the queries before
-  static constexpr int kFloats = kWarps * (kMeet + (kBf16 ? 0 : 8 * kRows));  // and fp32: weights of a part
+  static constexpr int kMeet = H * (kPitch + 2) + 7 & ~7;  // of a warp: outputs, maxima, sums; fp32: the queries before
+  static constexpr int kFloats = kWarps * (kMeet + (kBf16 ? 0 : 2 * H * kRows));  // and fp32: weights of a part, each twice
   static constexpr int kLoaders = std::min(4, kWarps), kThreads = (kWarps + kLoaders) * 32;
   static constexpr int kStages = std::min(6, (int)((227 * 1024 - 1024 - 1536 - kFloats * 4) / kStage));
   static constexpr int kSmem = kStages * kStage + kFloats * 4 + 1024;
@@ -125,13 +128,13 @@ __device__ __forceinline__ float exp2_of(float x, float m) { return m == -INFINI
 
 // What a warp knows of its 8 query heads: running maximum (of scores in units of log2), sum, unnormalised output.
 // bf16: lane (g, j) = (lane / 4, lane % 4) has features 8 i + 2 j, + 1 of head g in rows g and g + 8 of accumulator i.
-template <typename T, int DP>
+template <typename T, int DP, int H>
 struct State;
 
 template <int DP>
-struct State<__nv_bfloat16, DP> {
+struct State<__nv_bfloat16, DP, 8> {
   using T = __nv_bfloat16;
-  using S = Shape<T, DP>;
+  using S = Shape<T, DP, 8>;
   static constexpr int kRows = S::kRows;
   static constexpr int kSteps = DP / 16, kTiles = DP / 8;
   uint32_t q[kSteps][2];
@@ -254,115 +257,137 @@ struct State<__nv_bfloat16, DP> {
   }
 };
 
-// fp32: 32 / kRows lanes share a token's score (groups of four features in turn); lane has features lane, lane + 32, ... of the output of every head
-template <int DP>
-struct State<float, DP> {
-  using S = Shape<float, DP>;
-  static constexpr int kRows = S::kRows, kSplit = 32 / kRows;
-  static constexpr int kCols = DP / 32;
-  float o[8][kCols];
-  float m[8], l[8];  // l: of this lane's token
+// fp32: 32 / kRows lanes share a token's score (groups of four features in turn); lane has features 2 lane, 2 lane + 1, 2 lane + 64, ... of the output of every head.
+// Multiply-adds are packed, two features at a time.
+template <int DP, int H>
+struct State<float, DP, H> {
+  using S = Shape<float, DP, H>;
+  static constexpr int kRows = S::kRows, kSplit = 32 / kRows, kPairs = DP / 64;
+  uint64_t o[H][kPairs];
+  float m[H], l[H];  // l: of this lane's token
+  float q[H][DP / 32];
 
-  float q[8][kCols];
   __device__ __forceinline__ void fetch_queries(const Args& a, int req, int unit, int) {
     const int lane = threadIdx.x & 31;
     const Heads of(a, unit);
     const float* src = reinterpret_cast<const float*>(a.q) + req * a.q_req + (int64_t)of.first * a.q_head + lane;
 #pragma unroll
-    for (int g = 0; g < 8; ++g)
+    for (int g = 0; g < H; ++g)
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) q[g][c] = g < of.count && lane + 32 * c < a.d ? src[g * a.q_head + 32 * c] * a.scale_log2 : 0.f;
+      for (int c = 0; c < DP / 32; ++c) q[g][c] = g < of.count && lane + 32 * c < a.d ? src[g * a.q_head + 32 * c] * a.scale_log2 : 0.f;
   }
   __device__ __forceinline__ void share_queries(float* qs) const {  // in the warp
     const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int g = 0; g < 8; ++g)
+    for (int g = 0; g < H; ++g)
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) qs[g * DP + c * 32 + lane] = q[g][c];
+      for (int c = 0; c < DP / 32; ++c) qs[g * DP + c * 32 + lane] = q[g][c];
     __syncwarp();
   }
   __device__ __forceinline__ void begin() {
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
+    for (int g = 0; g < H; ++g) {
       m[g] = -INFINITY;
       l[g] = 0.f;
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) o[g][c] = 0.f;
+      for (int c = 0; c < kPairs; ++c) o[g][c] = 0;
     }
   }
-  __device__ __forceinline__ static float4 at(uint32_t from) {
-    float4 r;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"(from) : "memory");
-    return r;
+  __device__ __forceinline__ static void at(uint32_t from, uint64_t& x, uint64_t& y) {
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(x), "=l"(y) : "r"(from) : "memory");
   }
-  __device__ __forceinline__ static float one_at(uint32_t from) {
-    float r;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(from) : "memory");
+  __device__ __forceinline__ static uint64_t pair_at(uint32_t from) {
+    uint64_t r;
+    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(r) : "r"(from) : "memory");
     return r;
   }
   __device__ __forceinline__ void add(const Args& a, uint32_t keys, uint32_t vals, uint32_t bits, const float* qs, float* ps) {
-    const int lane = threadIdx.x & 31, t = lane & (kRows - 1), half = lane / kRows;
-    float s[8] = {};
+    const int lane = threadIdx.x & 31, t = lane & (kRows - 1), part = lane / kRows;
+    uint64_t s[H][2] = {};
+    const uint32_t qa = smem_u32(qs), pa = smem_u32(ps);
 #pragma unroll 4
-    for (int c = half; c < DP / 4; c += kSplit) {  // pieces of four features
-      const float4 k = at(keys + (c >> 3) * (kRows * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4));
+    for (int c = part; c < DP / 4; c += kSplit) {  // pieces of four features
+      uint64_t k0, k1;
+      at(keys + (c >> 3) * (kRows * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4), k0, k1);
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        if (g < a.unit_heads) {
-          const float4 q = *reinterpret_cast<const float4*>(qs + g * DP + c * 4);
-          s[g] += k.x * q.x + k.y * q.y + k.z * q.z + k.w * q.w;
-        }
+      for (int g = 0; g < H; ++g) {
+        uint64_t q0, q1;
+        at(qa + (g * DP + c * 4) * 4, q0, q1);
+        s[g][0] = fma2(k0, q0, s[g][0]);
+        s[g][1] = fma2(k1, q1, s[g][1]);
       }
     }
     const bool there = bits >> t & 1;
+    float x[H], top[H], f[H];
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      if (g >= a.unit_heads) continue;
-      float x = s[g];
+    for (int g = 0; g < H; ++g) {
+      float x0, x1;
+      split(add2(s[g][0], s[g][1]), x0, x1);
+      x[g] = x0 + x1;
+    }
 #pragma unroll
-      for (int w = kRows; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-      x = there ? x : -INFINITY;
-      float top = x;
+    for (int w = kRows; w < 32; w <<= 1)
 #pragma unroll
-      for (int w = 1; w < kRows; w <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, w));
-      const float mn = max_nan(m[g], top), f = exp2_of(m[g], mn), p = exp2_of(x, mn);
+      for (int g = 0; g < H; ++g) x[g] += __shfl_xor_sync(0xffffffffu, x[g], w);
+#pragma unroll
+    for (int g = 0; g < H; ++g) top[g] = x[g] = there ? x[g] : -INFINITY;
+#pragma unroll
+    for (int w = 1; w < kRows; w <<= 1)
+#pragma unroll
+      for (int g = 0; g < H; ++g) top[g] = max_nan(top[g], __shfl_xor_sync(0xffffffffu, top[g], w));
+    bool more = false;
+#pragma unroll
+    for (int g = 0; g < H; ++g) {
+      const float mn = max_nan(m[g], top[g]), p = exp2_of(x[g], mn);
+      f[g] = exp2_of(m[g], mn);
+      more |= f[g] != 1.f;
       m[g] = mn;
-      l[g] = l[g] * f + (half ? 0.f : p);
-      if (!half) ps[g * kRows + t] = p;
+      l[g] = l[g] * f[g] + (part ? 0.f : p);
+      if (!part) *reinterpret_cast<float2*>(ps + (g * kRows + t) * 2) = make_float2(p, p);
+    }
+    if (more) {  // (the same in all lanes)
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) o[g][c] *= f;
+      for (int g = 0; g < H; ++g)
+#pragma unroll
+        for (int c = 0; c < kPairs; ++c) o[g][c] = mul2(o[g][c], two(f[g], f[g]));
     }
     __syncwarp();
 #pragma unroll
     for (int t4 = 0; t4 < kRows; t4 += 4) {
-      float v[4][kCols];
+      uint64_t v[4][kPairs];
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) v[r][c] = one_at(vals + c * (kRows * 128) + (t4 + r) * 128 + (((lane >> 2) ^ ((t4 + r) & 7)) << 4) + (lane & 3) * 4);
+        for (int c = 0; c < kPairs; ++c) {
+          const int e = 64 * c + 2 * lane;
+          v[r][c] = pair_at(vals + (e >> 5) * (kRows * 128) + (t4 + r) * 128 + (((e >> 2 & 7) ^ ((t4 + r) & 7)) << 4) + (e & 3) * 4);
+        }
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        if (g >= a.unit_heads) continue;
-        const float4 p = *reinterpret_cast<const float4*>(ps + g * kRows + t4);
+      for (int g = 0; g < H; ++g) {
+        uint64_t p[4];
+        at(pa + (g * kRows + t4) * 8, p[0], p[1]);
+        at(pa + (g * kRows + t4 + 2) * 8, p[2], p[3]);
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) o[g][c] += p.x * v[0][c] + p.y * v[1][c] + p.z * v[2][c] + p.w * v[3][c];
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < kPairs; ++c) o[g][c] = fma2(p[r], v[r][c], o[g][c]);
       }
     }
     __syncwarp();
   }
   __device__ __forceinline__ void finish() {
 #pragma unroll
-    for (int g = 0; g < 8; ++g) l[g] = warp_sum(l[g]);
+    for (int g = 0; g < H; ++g) l[g] = warp_sum(l[g]);
   }
   __device__ __forceinline__ void give(float* to) const {
     const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
+    for (int g = 0; g < H; ++g) {
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) to[g * S::kPitch + c * 32 + lane] = o[g][c];
+      for (int c = 0; c < kPairs; ++c) *reinterpret_cast<uint64_t*>(to + g * S::kPitch + 64 * c + 2 * lane) = o[g][c];
       if (lane == 0) {
-        to[8 * S::kPitch + g] = m[g];
-        to[8 * S::kPitch + 8 + g] = l[g];
+        to[H * S::kPitch + g] = m[g];
+        to[H * S::kPitch + H + g] = l[g];
       }
     }
   }
@@ -375,12 +400,12 @@ __device__ __forceinline__ void put4<float>(float* to, float4 v) { *reinterpret_
 template <>
 __device__ __forceinline__ void put4<__nv_bfloat16>(__nv_bfloat16* to, float4 v) { *reinterpret_cast<uint2*>(to) = make_uint2(pack2(v.x, v.y), pack2(v.z, v.w)); }
 
-// MT: groups of 8 query heads in a unit. Multiplying warp (share, unit, m) has group m of the heads of a unit and MT parts of its tokens in a tile; the parts of a stage are
+// MT: groups of H query heads in a unit. Multiplying warp (share, unit, m) has group m of the heads of a unit and MT parts of its tokens in a tile; the parts of a stage are
 // ordered by unit and tokens
-template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(Shape<T, DP>::kThreads, 1)
+template <typename T, int DP, int MT, int H>
+__global__ void __launch_bounds__(Shape<T, DP, H>::kThreads, 1)
 attention_kernel(const Args a) {
-  using S = Shape<T, DP>;
+  using S = Shape<T, DP, H>;
   constexpr int kWarps = S::kWarps, kStages = S::kStages, kLoaders = S::kLoaders, kRows = S::kRows;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -569,7 +594,7 @@ attention_kernel(const Args a) {
   // ---- products
   const int m_tile = warp % MT, slot = warp / MT, shares = token_parts / MT, my_unit = slot % a.units, share = slot / a.units;
   float* box = boxes + warp * S::kMeet;  // of (share, unit, m)
-  float* ps = boxes + kWarps * S::kMeet + warp * 8 * kRows;
+  float* ps = boxes + kWarps * S::kMeet + warp * 2 * H * kRows;
   const uint32_t stages = smem_u32(smem);
   int meetings = 0;
   auto meet = [&]() {  // of the multiplying warps, where some have the same unit
@@ -578,7 +603,7 @@ attention_kernel(const Args a) {
     if (lane == 0) arrive(&meeting);
     ok = warp_wait(&meeting, meetings++ & 1, abort);
   };
-  State<T, DP> st;
+  State<T, DP, H> st;
   Place cur = start_shared;
   long long cost = cost_shared;  // where the present (request, group) begins
   st.fetch_queries(a, cur.req, cur.group * a.units + my_unit, m_tile);
@@ -630,15 +655,15 @@ attention_kernel(const Args a) {
     st.give(box);
     meet();
     if (!ok) break;
-    const int of = 8 * (DP / 4), all = shares == 1 ? of : of * MT * a.units;
+    const int of = H * (DP / 4), all = shares == 1 ? of : of * MT * a.units;
     for (int i = shares == 1 ? lane : threadIdx.x; i < all; i += shares == 1 ? 32 : kWarps * 32) {
-      const int e = i % (DP / 4) * 4, g = i / (DP / 4) % 8;
+      const int e = i % (DP / 4) * 4, g = i / (DP / 4) % H;
       int mt = m_tile, un = my_unit;
       if (shares != 1) {
         mt = i / of % MT;
         un = i / of / MT;
       }
-      const int h = mt * 8 + g;
+      const int h = mt * H + g;
       const Heads of_unit(a, done.group * a.units + un);
       if (e >= a.d || h >= of_unit.count) continue;
       const float* b = boxes + (un * MT + mt) * S::kMeet;
@@ -646,15 +671,15 @@ attention_kernel(const Args a) {
       float m = -INFINITY, l = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps / MT; ++w) {
-        if (w < shares) m = max_nan(m, b[w * pitch + 8 * S::kPitch + g]);
+        if (w < shares) m = max_nan(m, b[w * pitch + H * S::kPitch + g]);
       }
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps / MT; ++w) {
         if (w >= shares) break;
-        const float f = exp2_of(b[w * pitch + 8 * S::kPitch + g], m);
+        const float f = exp2_of(b[w * pitch + H * S::kPitch + g], m);
         const float4 x = *reinterpret_cast<const float4*>(b + w * pitch + g * S::kPitch + e);
-        l += b[w * pitch + 8 * S::kPitch + 8 + g] * f;
+        l += b[w * pitch + H * S::kPitch + H + g] * f;
         o.x += x.x * f;
         o.y += x.y * f;
         o.z += x.z * f;
@@ -742,9 +767,9 @@ join_kernel(const Args a) {
   }
 }
 
-template <typename T, int DP, int MT>
+template <typename T, int DP, int MT, int H>
 int launch(Args a, cudaStream_t stream) {
-  using S = Shape<T, DP>;
+  using S = Shape<T, DP, H>;
   a.whole = a.page % S::kRows == 0 && a.d == DP;
   const int slots = S::kWarps / MT;
   a.units = std::min(a.units, slots);
@@ -753,7 +778,7 @@ int launch(Args a, cudaStream_t stream) {
   a.group_cost = a.units == slots ? 1 : 2;
   static_assert(S::kStages >= 2 && S::kSmem + 1536 <= 227 * 1024, "shared memory");
   static RbPerDevice ready;
-  auto kernel = attention_kernel<T, DP, MT>;
+  auto kernel = attention_kernel<T, DP, MT, H>;
   if (ready.needed()) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess) return rb_check_launch("paged_attention");
     ready.done();
@@ -763,11 +788,11 @@ int launch(Args a, cudaStream_t stream) {
   return rb_check_launch("paged_attention");
 }
 
-template <typename T, int MT>
+template <typename T, int MT, int H>
 int by_dim(const Args& a, cudaStream_t stream) {
-  if (a.d <= 64) return launch<T, 64, MT>(a, stream);
-  if (a.d <= 128) return launch<T, 128, MT>(a, stream);
-  return launch<T, 256, MT>(a, stream);
+  if (a.d <= 64) return launch<T, 64, MT, H>(a, stream);
+  if (a.d <= 128) return launch<T, 128, MT, H>(a, stream);
+  return launch<T, 256, MT, H>(a, stream);
 }
 
 int units_of(int group, int bf16, int* unit_heads) {
@@ -823,8 +848,12 @@ RB_EXPORT int rb200_paged_attention(const void* q, const void* k, const void* v,
   a.cuts = reinterpret_cast<int4*>(workspace);
   a.part = reinterpret_cast<float*>(a.cuts + a.grid);
   a.units = group_of(n, kv_heads * a.units_per_kv);
-  if (!bf16) return by_dim<float, 1>(a, stream);
-  if (a.unit_heads <= 8) return by_dim<__nv_bfloat16, 1>(a, stream);
-  if (a.unit_heads <= 16) return by_dim<__nv_bfloat16, 2>(a, stream);
-  return by_dim<__nv_bfloat16, 4>(a, stream);
+  if (!bf16) {
+    if (a.unit_heads == 1) return by_dim<float, 1, 1>(a, stream);
+    if (a.unit_heads == 2) return by_dim<float, 1, 2>(a, stream);
+    return a.unit_heads <= 4 ? by_dim<float, 1, 4>(a, stream) : by_dim<float, 1, 8>(a, stream);
+  }
+  if (a.unit_heads <= 8) return by_dim<__nv_bfloat16, 1, 8>(a, stream);
+  if (a.unit_heads <= 16) return by_dim<__nv_bfloat16, 2, 8>(a, stream);
+  return by_dim<__nv_bfloat16, 4, 8>(a, stream);
 }
