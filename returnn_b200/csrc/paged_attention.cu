@@ -8,7 +8,7 @@
 // A unit is a key head with up to 8 * MT of its query heads. A tile is the parts of 16 tokens of the multiplying warps: of one unit, or of fewer tokens of 2, 4 or 8
 // units where there are enough requests. Warps of one unit bring their outputs together at its end; with a unit for each warp there is nothing to bring
 // together, and requests of a few tokens fill the warps (see group_of).
-// Within a CTA four warps look the pages up and send for them, several tiles ahead, also across the end of a (request, unit); the others multiply, 16 tokens of a
+// Within a CTA four or eight warps look the pages up and send for them, several tiles ahead, also across the end of a (request, unit); the others multiply, 16 tokens of a
 // tile each, which are waited for and refilled by themselves. Rows beyond the length are filled with zeros and not read. The copies are the 16-byte
 // asynchronous ones of the loading warps' lanes, which take any page size and any strides: boxes of 16 tokens x 128 bytes by TMA were issued and fetched at
 // 5.0 to 5.9 TB/s without any product behind them, and boxes cannot be larger where a page holds 16 tokens.
@@ -60,7 +60,11 @@ struct Shape {
   static constexpr int kPitch = DP + 8;              // floats of a head where the warps meet (no bank conflicts)
   static constexpr int kMeet = H * (kPitch + 2) + 7 & ~7;  // of a warp: outputs, maxima, sums; fp32: the queries before
   static constexpr int kFloats = kWarps * (kMeet + (kBf16 ? 0 : 2 * H * kRows));  // and fp32: weights of a part, each twice
-  static constexpr int kLoaders = std::min(4, kWarps), kThreads = (kWarps + kLoaders) * 32;
+  // loading warps: what they issue sets the pace of rows of 128 bytes with one group of heads (28 requests, 112680 tokens, 12 heads of 64, bf16: 68.4 us with four, 64.2 with eight; 64 over
+  // 4 heads 33.5 and 36.1) and of four heads over parts of 8 rows (32 over 8 heads of 128, fp32: 165 and 152). Elsewhere four are enough and leave the registers
+  // (32 over 8 of 128, bf16: 73.5 and 76.6).
+  static constexpr int loaders(int mt) { return (kBf16 && kRowBytes == 128 && mt == 1) || (!kBf16 && kRowBytes == 512 && H == 4) ? 8 : std::min(4, kWarps); }
+  static constexpr int threads(int mt) { return (kWarps + loaders(mt)) * 32; }
   static constexpr int kStages = std::min(6, (int)((227 * 1024 - 1024 - 1536 - kFloats * 4) / kStage));
   static constexpr int kSmem = kStages * kStage + kFloats * 4 + 1024;
 };
@@ -403,10 +407,10 @@ __device__ __forceinline__ void put4<__nv_bfloat16>(__nv_bfloat16* to, float4 v)
 // MT: groups of H query heads in a unit. Multiplying warp (share, unit, m) has group m of the heads of a unit and MT parts of its tokens in a tile; the parts of a stage are
 // ordered by unit and tokens
 template <typename T, int DP, int MT, int H>
-__global__ void __launch_bounds__(Shape<T, DP, H>::kThreads, 1)
+__global__ void __launch_bounds__(Shape<T, DP, H>::threads(MT), 1)
 attention_kernel(const Args a) {
   using S = Shape<T, DP, H>;
-  constexpr int kWarps = S::kWarps, kStages = S::kStages, kLoaders = S::kLoaders, kRows = S::kRows;
+  constexpr int kWarps = S::kWarps, kStages = S::kStages, kLoaders = S::loaders(MT), kRows = S::kRows;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   float* boxes = reinterpret_cast<float*>(smem + kStages * S::kStage);
@@ -783,7 +787,7 @@ int launch(Args a, cudaStream_t stream) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess) return rb_check_launch("paged_attention");
     ready.done();
   }
-  rb_launch_pdl(kernel, dim3(a.grid), dim3(S::kThreads), (size_t)S::kSmem, stream, a);
+  rb_launch_pdl(kernel, dim3(a.grid), dim3(S::threads(MT)), (size_t)S::kSmem, stream, a);
   rb_launch_pdl(join_kernel<T>, dim3(a.grid, (a.units * a.unit_heads + kJoin - 1) / kJoin), dim3(kJoin * 32), 0, stream, a);
   return rb_check_launch("paged_attention");
 }
