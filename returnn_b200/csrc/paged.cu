@@ -291,10 +291,11 @@ RB_EXPORT int rb200_paged_append(int* table, long long table_stride, int blocks,
                                  long long* new_range, void* granted, cudaStream_t stream) {
   if (bad("paged_append", n, blocks, ring_size, page) || max_tokens < 0) return RB_ERR_ARG;
   // A token per thread where that is a wave of CTAs, four beyond; a request per thread where they fit one round. Device us, 64 requests of one token 3.4, with four
-  // tokens a thread 5.0, with four requests a thread 4.1; 1M tokens of 256 requests (12 MB of lists, bound by the searches and the trip to the table) 9.7, with a token a
-  // thread 14.7, of 500 requests 12.2 and 23.8
+  // tokens a thread 5.0, with four requests a thread 4.1; 1M tokens of 256 requests (12 MB of lists, bound by the searches and the trip to the table) 9.0, with a token a
+  // thread 14.7, of 500 requests 12.2 and 23.8. Eight CTAs to an
+  // SM, or four where each goes over more requests than it has threads (the same 1M tokens with four and eight: 9.7 and 9.0, of 500 requests 12.2 and 16.1)
   const bool four = max_tokens > 148 * kThreads, many = n > kThreads;
-  const long long of = (four ? 4 : 1) * kThreads, ctas = std::min<long long>(std::max<long long>((max_tokens + of - 1) / of, 1), 148 * 4);
+  const long long of = (four ? 4 : 1) * kThreads, ctas = std::min<long long>(std::max<long long>((max_tokens + of - 1) / of, 1), 148 * (many ? 4 : 8));
   auto kernel = many ? (four ? append_kernel<4, 4> : append_kernel<4, 1>) : (four ? append_kernel<1, 4> : append_kernel<1, 1>);
   rb_launch_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), 0, stream, table, table_stride, blocks, lens, add, n, Ring{ring, ring_size}, range, page_of(page),
                 max_tokens, slots, positions, requests, offsets, new_lens, new_range, reinterpret_cast<uint8_t*>(granted));

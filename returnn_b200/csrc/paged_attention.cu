@@ -732,6 +732,10 @@ join_kernel(const Args a) {
   float4 acc[2] = {};
   for (int c0 = began; c0 <= cut.z; c0 += 32) {
     const int count = min(32, cut.z + 1 - c0);
+    constexpr int kAhead = 8;  // outputs that are under way with the maxima
+    float4 ahead[kAhead];
+#pragma unroll
+    for (int c = 0; c < kAhead; ++c) ahead[c] = c < count && lane * 4 < a.d ? *reinterpret_cast<const float4*>(part(c0 + c) + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
     float mine = -INFINITY, sum = 0.f;
     if (lane < count) {
       const float2 x = *reinterpret_cast<const float2*>(part(c0 + lane) + a.d);
@@ -746,20 +750,25 @@ join_kernel(const Args a) {
     l = l * old + warp_sum(sum * f);
 #pragma unroll
     for (int k = 0; k < 2; ++k) acc[k] = make_float4(acc[k].x * old, acc[k].y * old, acc[k].z * old, acc[k].w * old);
-#pragma unroll 8
-    for (int c = 0; c < count; ++c) {
-      const float* p = part(c0 + c);
-      const float fc = __shfl_sync(0xffffffffu, f, c);
+    auto weigh = [&](float4& to, const float4& x, float by) {
+      to.x += x.x * by;
+      to.y += x.y * by;
+      to.z += x.z * by;
+      to.w += x.w * by;
+    };
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int e = (lane + 32 * k) * 4;
-        if (e < a.d) {
-          const float4 x = *reinterpret_cast<const float4*>(p + e);
-          acc[k].x += x.x * fc;
-          acc[k].y += x.y * fc;
-          acc[k].z += x.z * fc;
-          acc[k].w += x.w * fc;
-        }
+    for (int c = 0; c < kAhead; ++c)
+      if (c < count) weigh(acc[0], ahead[c], __shfl_sync(0xffffffffu, f, c));
+#pragma unroll 8
+    for (int c = kAhead; c < count; ++c) {
+      const float fc = __shfl_sync(0xffffffffu, f, c);
+      if (lane * 4 < a.d) weigh(acc[0], *reinterpret_cast<const float4*>(part(c0 + c) + lane * 4), fc);
+    }
+    if (a.d > 128) {
+#pragma unroll 8
+      for (int c = 0; c < count; ++c) {
+        const float fc = __shfl_sync(0xffffffffu, f, c);
+        if (lane * 4 + 128 < a.d) weigh(acc[1], *reinterpret_cast<const float4*>(part(c0 + c) + lane * 4 + 128), fc);
       }
     }
   }
