@@ -315,12 +315,14 @@ forward_kernel(const Args a) {
   const int rest = a.v - (r.v8 - r.head);  // fewer than the threads
   if ((int)threadIdx.x < rest) xr = ld(a.x, r.base + ((int)threadIdx.x < r.head ? threadIdx.x : threadIdx.x + (r.v8 - r.head)), kBf16);
   Stat st{-INFINITY, 0.f, 0.f};
-  for (int64_t c0 = r.head + (int)threadIdx.x * kN; c0 < r.v8; c0 += kBatch * kThreads * kN) {
+  // kAll: every piece lies in the row
+  auto batch = [&](int64_t c0, auto all) {
+    constexpr bool kAll = decltype(all)::value;
     Chunk<kBf16> u[kBatch];
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) {
       const int64_t c = c0 + q * kThreads * kN;
-      if (c < r.v8) u[q].load(a.x, r.base + c);
+      if (kAll || c < r.v8) u[q].load(a.x, r.base + c);
       else u[q].fill_neg_inf();
     }
     float lm = u[0].max();
@@ -334,7 +336,7 @@ forward_kernel(const Args a) {
       uint64_t s = 0, w = 0;
 #pragma unroll
       for (int q = 0; q < kBatch; ++q) {
-        if (q == 0 || c0 + q * kThreads * kN < r.v8) {
+        if (kAll || q == 0 || c0 + q * kThreads * kN < r.v8) {
           uint64_t p[kN / 2];
           in_pairs<kEntropy>(u[q], least, p);
 #pragma unroll
@@ -358,10 +360,16 @@ forward_kernel(const Args a) {
     } else {
 #pragma unroll
       for (int q = 0; q < kBatch; ++q)
-        if (q == 0 || c0 + q * kThreads * kN < r.v8)
+        if (kAll || q == 0 || c0 + q * kThreads * kN < r.v8)
           for (int k = 0; k < kN; ++k) add<kEntropy>(u[q].at(k), m, st.s, st.w);
     }
-  }
+  };
+  int64_t c0 = r.head + (int)threadIdx.x * kN;
+  // whole batches without a check for each piece, where registers allow the second copy of the body (4 x 128000 fp32, 8 best: 10.7 and 9.5 us; with 128 threads, 6001 x 10001
+  // fp32, 40.2 and 42.2)
+  if (kThreads != 128)
+    for (; c0 + (kBatch - 1) * kThreads * kN < r.v8; c0 += kBatch * kThreads * kN) batch(c0, std::true_type());
+  for (; c0 < r.v8; c0 += kBatch * kThreads * kN) batch(c0, std::false_type());
   if ((int)threadIdx.x < rest) {
     if (xr > st.m) st.to(xr);
     add<kEntropy>(xr, st.m == -INFINITY ? 0.f : st.m, st.s, st.w);
@@ -577,8 +585,8 @@ RB_EXPORT int rb200_token_log_probs_fwd(const void* x, long long pitch, const vo
   a.top_label = top_label;
   // Threads of a row and 16-byte pieces that each has under way. Many rows: 128, 12 rows on an SM, where the latencies of one row's end are hidden best (us with 128 and 256:
   // 1500 x 10001 fp32, 8 best 15.9 and 18.3; 6001 x 32000 bf16 70.7 and 69.7, with 8 best 86.9 and 86.7). Fewer do not fill the SMs so: 256 (850 x 32000 fp32, 32 best: 38.5
-  // and 28.1), and twice the pieces where four rows on an SM are all (500 x 32000: 12.9, with more pieces 9.4; 486 x 128000, 5 best: 46.4 and 32.9). With two rows on an SM or
-  // fewer, 1024 threads for many labels (16 x 32000, 5 best: 6.8 with 256, 5.6; 4 x 128000 fp32, 8 best: 21.2 and 10.9; but 183 x 10001, 32 best, with gradient 11.7 and 19.6).
+  // and 28.1), and twice the pieces where four rows on an SM are all (500 x 32000: 12.9, with more pieces 9.4; 486 x 128000, 5 best: 46.4 and 30.5). With two rows on an SM or
+  // fewer, 1024 threads for many labels (16 x 32000, 5 best: 6.8 with 256, 5.4; 4 x 128000 fp32, 8 best: 21.2 and 9.5; but 183 x 10001, 32 best, with gradient 11.7 and 19.6).
   const int way = rows >= 8 * 148 ? 0 : v < 8192 || rows > 4 * 148 ? 1 : rows > 2 * 148 || v < 16384 ? 2 : 3;
   auto pick = [&](auto threads, auto batch, auto b) {
     constexpr int kT = decltype(threads)::value, kP = decltype(batch)::value;
