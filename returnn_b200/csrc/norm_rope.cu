@@ -10,7 +10,7 @@
 // Rows are read once and written once. A row of D features sits in the next power of two of D / 8 lanes, 8 features a lane, chosen so that both features of a pair
 // are the lane's own: 8 in a row for pairs (2i, 2i + 1), 4 of each half for pairs (i, i + R / 2). The mean is a few shuffles. Head dims, rotated parts and
 // alignments that do not fit this take a warp per row with single elements.
-// Measured, both passes with the norm: 25000 x 16 heads of 64, bf16, 256 MB, 62.7 us (4.1 TB/s; a copy of as many bytes takes 42), bound by the instructions of a row of 128
+// Measured, both passes with the norm: 25000 x 16 heads of 64, bf16, 256 MB, 61.8 us (4.1 TB/s; a copy of as many bytes takes 42), bound by the instructions of a row of 128
 // bytes; 8191 x 40 of 128, fp32, 839 MB, 138.5 us (6.1 TB/s, what the memory gives).
 #include "packed_f32.cuh"
 #include <algorithm>
@@ -634,17 +634,20 @@ bool fits(const Args& a, int bf16, bool backward, bool cache) {
   return ok;
 }
 
-// A tile is as many tokens as fill the table with an angle per thread; fewer where that leaves SMs without any. A CTA of the backward pass has one tile after another, each with a
-// beginning that costs about as much as two rows of a group: tiles are up to four times as large where the turns that all tiles take are the shorter for it (8191 tokens x 40
-// rows of 128, bf16, both passes: 103.6 us with 4 tokens, 97.1 with 16; 20000 x 24 of 64 take 8, 5 turns of which are shorter than 3 of 16). Where all tiles are on the SMs at once, their heads are shared by
-// as many CTAs as it takes for every group to have one head (returned): all rows are then asked for at the beginning.
-int tile_of(Args& a, int rows, int groups, int ctas, bool backward) {
+// A tile is as many tokens as fill the table with an angle per thread; fewer where that leaves SMs without any. Each has a beginning that costs about as much as two rows of a group:
+// tiles are up to four times as large where the turns in which the SMs take them are the shorter for it (bf16, us, 8191 tokens x 40 rows of 128, both passes: 103.6 with 4 tokens,
+// 97.1 with 16 in the backward pass; forward 38.3 and 35.6; 100000 x 40 of 128 forward 405 and 364; 20000 x 24 of 64 take 8: 5 turns of those are shorter than 3 of 16, 26.6 and
+// 34.6). Not so for fp32 forward, whose rows are bound by the memory (8191 x 40 of 128: 56 and 64), nor for a turn and a half (6000 x 16 of 64: 7.4 and 8.4).
+// Where all tiles are on the SMs at once, their heads are shared by as many CTAs as it takes for every group to have one head (returned): all rows are then asked for at the
+// beginning.
+int tile_of(Args& a, int rows, int groups, int ctas, bool may_grow) {
   const int need = std::max(1, (rows + groups - 1) / groups);
   auto tiles = [&]() { return (a.n + a.tokens - 1) / a.tokens; };
   a.tokens = a.rot ? std::max(1, kThreads / (a.rot / 2)) : 8;
-  if (backward) {
+  const int64_t slots = ctas * 148;
+  if (may_grow && tiles() * 2 >= slots * 3) {
     const int least = a.tokens;
-    auto turns = [&]() { return ((tiles() + ctas * 148 - 1) / (ctas * 148)) * (a.tokens * (int64_t)rows + 2 * groups); };
+    auto turns = [&]() { return (tiles() + slots - 1) / slots * (a.tokens * (int64_t)rows + 2 * groups); };
     int best = least;
     int64_t cost = turns();
     for (int more = 2; more <= 4; more *= 2) {
@@ -674,7 +677,7 @@ int forward(Args& a, int bf16, bool cache, cudaStream_t stream) {
   if (a.n <= 0 || rows == 0) return RB_OK;
   a.inv_d = 1.f / a.d;
   if (fits(a, bf16, false, cache)) {
-    const int gy = tile_of(a, rows, kThreads / lanes_of(a.d), bf16 ? kCtasBf16 : kCtasF32, false);
+    const int gy = tile_of(a, rows, kThreads / lanes_of(a.d), bf16 ? kCtasBf16 : kCtasF32, bf16);
     const int64_t gx = (a.n + a.tokens - 1) / a.tokens;
     if (gx > 0x7fffffff) {
       rb_set_error("norm_rope: %lld tokens", (long long)a.n);
