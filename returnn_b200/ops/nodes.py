@@ -63,3 +63,14 @@ def active():
 def launches() -> int:
     """number of kernels that the nodes launched so far"""
     return _module.launches() if _module is not None else 0
+
+
+def of(tensor):
+    """
+    :return: :func:`active` where the native kernels run for ``tensor``, else None. One short call in front of operators that take a few microseconds.
+    """
+    if not tensor.is_cuda:
+        return None
+    if _lib._lib is None or _lib._env_data.get(b"RETURNN_B200_DISABLE_NATIVE", b"0") == b"1":
+        return active() if _lib.use_native(tensor) else None
+    return active()

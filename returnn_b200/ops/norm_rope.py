@@ -194,12 +194,11 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tensor
     :param k_scale: [D] scale of the norm of the keys
     :return: rotated q and k, contiguous
     """
-    if q.is_cuda and _lib.use_native(q):
-        mod = nodes.active()
-        if mod is not None:
-            res = mod.norm_rope(q, k, positions, frequencies, q_scale, k_scale, eps, interleaved, amplitude)
-            if res is not None:
-                return res
+    mod = nodes.of(q)
+    if mod is not None:
+        res = mod.norm_rope(q, k, positions, frequencies, q_scale, k_scale, eps, interleaved, amplitude)
+        if res is not None:
+            return res
     _check(q, k, positions, frequencies, q_scale, k_scale, "norm_rope")
     if _native_ok(q, q_scale, "norm_rope"):
         return _NormRopeFn.apply(q, k, positions, frequencies, q_scale, k_scale, float(eps), bool(interleaved), float(amplitude))
@@ -223,12 +222,11 @@ def norm_rope_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positi
     :return: rotated q [N, heads, D]
     """
     what = "norm_rope_to_cache"
-    if q.is_cuda and _lib.use_native(q):
-        mod = nodes.active()
-        if mod is not None:
-            res = mod.norm_rope_to_cache(q, k, v, k_cache, v_cache, slots, positions, frequencies, q_scale, k_scale, eps, interleaved, amplitude)
-            if res is not None:
-                return res
+    mod = nodes.of(q)
+    if mod is not None:
+        res = mod.norm_rope_to_cache(q, k, v, k_cache, v_cache, slots, positions, frequencies, q_scale, k_scale, eps, interleaved, amplitude)
+        if res is not None:
+            return res
     _check(q, k, positions, frequencies, q_scale, k_scale, what)
     if q.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError("%s: q %s, k %s, v %s %s must be [N, heads, D] of one type" % (what, tuple(q.shape), tuple(k.shape), tuple(v.shape), v.dtype))

@@ -83,12 +83,11 @@ def append_tokens(block_table: torch.Tensor, lengths: torch.Tensor, counts: torc
     :param max_tokens: room for new tokens, at least ``counts.sum()`` (tokens beyond it are left out of the lists, not of the lengths)
     """
     what = "append_tokens"
-    if block_table.is_cuda and _lib.use_native(block_table):
-        mod = nodes.active()
-        if mod is not None:
-            res = mod.append_tokens(block_table, lengths, counts, free_pages, free_range, page_size, max_tokens)
-            if res is not None:
-                return AppendedTokens(*res)
+    mod = nodes.of(block_table)
+    if mod is not None:
+        res = mod.append_tokens(block_table, lengths, counts, free_pages, free_range, page_size, max_tokens)
+        if res is not None:
+            return AppendedTokens(*res)
     _check_table(what, block_table, lengths, counts, torch.int32, free_pages, free_range, page_size)
     if max_tokens < 0:
         raise ValueError("%s: max_tokens %r" % (what, max_tokens))
@@ -121,12 +120,11 @@ def release_pages(block_table: torch.Tensor, lengths: torch.Tensor, finished: to
     :param finished: [requests] bool
     """
     what = "release_pages"
-    if block_table.is_cuda and _lib.use_native(block_table):
-        mod = nodes.active()
-        if mod is not None:
-            res = mod.release_pages(block_table, lengths, finished, free_pages, free_range, page_size)
-            if res is not None:
-                return ReleasedPages(*res)
+    mod = nodes.of(block_table)
+    if mod is not None:
+        res = mod.release_pages(block_table, lengths, finished, free_pages, free_range, page_size)
+        if res is not None:
+            return ReleasedPages(*res)
     _check_table(what, block_table, lengths, finished, torch.bool, free_pages, free_range, page_size)
     if not (block_table.is_cuda and _lib.use_native(block_table)):
         return release_pages_reference(block_table, lengths, finished, free_pages, free_range, page_size=page_size)
@@ -158,12 +156,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     :return: [requests, heads, D], contiguous
     """
     what = "paged_attention"
-    if q.is_cuda and _lib.use_native(q):
-        mod = nodes.active()
-        if mod is not None:
-            res = mod.paged_attention(q, k_cache, v_cache, block_table, lengths, q.shape[-1] ** -0.5 if scale is None else scale, status_tensor(q.device))
-            if res is not None:
-                return res
+    mod = nodes.of(q)
+    if mod is not None:
+        res = mod.paged_attention(q, k_cache, v_cache, block_table, lengths, q.shape[-1] ** -0.5 if scale is None else scale, status_tensor(q.device))
+        if res is not None:
+            return res
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[3] != q.shape[2]:
         raise ValueError("%s: q %s must be [requests, heads, D], the caches [pages, key heads, page size, D], got %s and %s" % (
             what, tuple(q.shape), tuple(k_cache.shape), tuple(v_cache.shape)))

@@ -87,12 +87,11 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, *, entropy: boo
     :param num_top: also that many best labels, at most 32 and at most V
     """
     what = "token_log_probs"
-    if logits.is_cuda and _lib.use_native(logits):
-        mod = nodes.active()
-        if mod is not None:
-            res = mod.token_log_probs(logits, targets, entropy, num_top)
-            if res is not None:
-                return TokenLogProbs(*res)
+    mod = nodes.of(logits)
+    if mod is not None:
+        res = mod.token_log_probs(logits, targets, entropy, num_top)
+        if res is not None:
+            return TokenLogProbs(*res)
     if logits.dim() != 2 or targets.shape != logits.shape[:1]:
         raise ValueError("%s: logits %s must be [rows, V], targets %s [rows]" % (what, tuple(logits.shape), tuple(targets.shape)))
     if targets.dtype not in (torch.int32, torch.int64) or targets.device != logits.device:
