@@ -583,11 +583,19 @@ RB_EXPORT int rb200_token_log_probs_fwd(const void* x, long long pitch, const vo
   Args a = {};
   a.x = x; a.pitch = pitch; a.target = target; a.target64 = target64; a.v = v; a.top = top; a.lp = lp; a.norm = norm; a.entropy = entropy; a.top_lp = top_lp;
   a.top_label = top_label;
-  // Threads of a row and 16-byte pieces that each has under way. Many rows: 128, 12 rows on an SM, where the latencies of one row's end are hidden best (us with 128 and 256:
-  // 1500 x 10001 fp32, 8 best 15.9 and 18.3; 6001 x 32000 bf16 70.7 and 69.7, with 8 best 86.9 and 86.7). Fewer do not fill the SMs so: 256 (850 x 32000 fp32, 32 best: 38.5
-  // and 28.1), and twice the pieces where four rows on an SM are all (500 x 32000: 12.9, with more pieces 9.4; 486 x 128000, 5 best: 46.4 and 30.5). With two rows on an SM or
-  // fewer, 1024 threads for many labels (16 x 32000, 5 best: 6.8 with 256, 5.4; 4 x 128000 fp32, 8 best: 21.2 and 9.5; but 183 x 10001, 32 best, with gradient 11.7 and 19.6).
-  const int way = rows >= 8 * 148 ? 0 : v < 8192 || rows > 4 * 148 ? 1 : rows > 2 * 148 || v < 16384 ? 2 : 3;
+  // Threads of a row and 16-byte pieces that each has under way: 128 with four pieces (12 rows on an SM), 256 with four (six) or eight (four), 1024. Measured, us:
+  // many rows, below 48 KB each: 128, where the latencies of one row's end are hidden best (1500 x 10001 fp32, 8 best: 15.9, with 256 18.3; 2740 x 1001, 20 best 12.5 and 23.5);
+  // many longer rows: 256 (6001 x 32000 fp32, 32 best: with 128 222, 164), with eight pieces unless the ends of the rows are the longer (2000 x 128000 bf16, 8 best: with 128 132,
+  // four pieces 106, eight 97; 6001 x 32000 bf16, 8 best: 89, 82, 86);
+  // rows that are all on the SMs at once: as many pieces as that leaves room for (800 x 50001 fp32, 8 best: four 31, eight 36; 500 x 32000 bf16: 12.9 and 9.2);
+  // two rows on an SM or fewer: 1024 for many labels (16 x 32000, 5 best: 6.8 with 256, 5.4; 4 x 128000 fp32, 8 best: 21.2 and 9.5; but 183 x 10001, 32 best, with
+  // gradient 11.7 and 19.6).
+  const long long bytes = (long long)v * (bf16 ? 2 : 4);
+  const int way = rows <= 2 * 148   ? (v < 8192 ? 1 : v < 16384 ? 2 : 3)
+                  : rows <= 4 * 148 ? (v < 8192 ? 1 : 2)
+                  : rows <= 6 * 148 ? 1
+                  : bytes >= (48 << 10) ? (top && bytes < (128 << 10) ? 1 : 2)
+                                        : (rows >= 8 * 148 ? 0 : 1);
   auto pick = [&](auto threads, auto batch, auto b) {
     constexpr int kT = decltype(threads)::value, kP = decltype(batch)::value;
     constexpr bool kB = decltype(b)::value;
