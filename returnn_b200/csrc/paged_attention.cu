@@ -17,10 +17,10 @@
 // larger tensor-memory instructions have nothing to win (64 rows at least, keys would pass through descriptors) and the sixteen rows here are only half used:
 // rows 0..7 are 8 query heads with the weights rounded to bf16, rows 8..15 the same heads with what the rounding lost. Their sum weighs the
 // values with 16 bits of mantissa at no further instruction; weights of 8 bits would add an error as large as the rounding of the result.
-// fp32: products by fused multiply-adds, a kernel for 1, 2, 4 and 8 heads of a unit (14 requests, 56340 tokens, D 128, 4 on each of 8 key heads: 89 us; with one kernel and the heads
+// fp32: products by fused multiply-adds, a kernel for 1, 2, 4 and 8 heads of a unit (14 requests, 56340 tokens, D 128, 4 on each of 8 key heads: 88 us; with one kernel and the heads
 // counted at run time 169).
-// Measured (D 128, 4 query heads on each of 8 key heads, bf16): 64 requests of 122637 tokens together, 502 MB, 85 us (5.9 TB/s); two of 76484 and 131072, 850 MB, 133 us
-// (6.4 TB/s). Small calls are the launches and the chain of length, page, token, product and join: one request of 1000 tokens, fp32, D 64, 9.1 us.
+// Measured (D 128, 4 query heads on each of 8 key heads, bf16): 64 requests of 122637 tokens together, 502 MB, 85 us (5.9 TB/s); two of 76484 and 131072, 850 MB, 132 us
+// (6.4 TB/s). Small calls are the launches and the chain of length, page, token, product and join: one request of 1000 tokens, fp32, D 64, 8.2 us.
 #include "packed_f32.cuh"
 #include "tcgen05.cuh"
 #include <algorithm>
@@ -709,7 +709,7 @@ attention_kernel(const Args a) {
   }
 }
 
-// joins the parts of a (request, group) that several CTAs had: block (c, y) the one that CTA c began (two requests of 5615 tokens, two units: 17 us with the pass; a thread
+// joins the parts of a (request, group) that several CTAs had: block (c, y) the one that CTA c began (two requests of 5615 tokens, two units: 14 us with the pass; a thread
 // per feature, part after part, took 27). A warp per query head: its lanes weigh a part each, then take
 // four features each of all parts, several under way at a time.
 template <typename T>
@@ -818,7 +818,7 @@ int units_of(int group, int bf16, int* unit_heads) {
 }  // namespace
 
 // units of a group: a power of two that divides the units, with which there is still a (request, group) for every other SM. Measured (bf16, 8 units) with 1, 2, 4 and 8:
-// 378 requests of up to 11 tokens 54, 42, 30, 18 us; 64 of up to 4096 84.5, 83.7, 84.7, 87.6; 4 of up to 920 11.0, 12.1, 18.1, 25.1.
+// 378 requests of up to 11 tokens 57, 35, 24, 17 us; 64 of up to 4096 84.2, 83.7, 84.9, 85.9; 4 of up to 920 10.1, 10.7, 13.4, 15.8.
 static int group_of(int n, int units) {
   int g = 1;
   while (g < 8 && units % (2 * g) == 0 && (long long)n * units / (2 * g) >= num_sms() / 2) g *= 2;
