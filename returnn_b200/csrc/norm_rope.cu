@@ -380,7 +380,8 @@ backward_kernel(const Args a) {
             if (live && l.turned) rotate4(g, table + tk * a.rot + l.sub * 8);
             if (kNorm) {
               const P4 x = raw_x[u].get();
-              const float inv = rsqrtf(group_sum(dot_of(x, x), kLanes) * a.inv_d + a.eps);
+              const float square = group_sum(dot_of(x, x), kLanes) * a.inv_d + a.eps;
+              const float inv = turn.mine && tk < nt ? rsqrtf(square) : 0.f;  // (no row here: without an epsilon the zeros would have no norm)
               const P4 v = scaled(x, inv);
 #pragma unroll
               for (int j = 0; j < 4; ++j) sum.v[j] = fma2(g.v[j], v.v[j], sum.v[j]);  // (zeros in lanes and groups without a row)

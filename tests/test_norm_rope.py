@@ -260,3 +260,26 @@ def test_refusals(device):
         big = torch.zeros(1, 1, 258, device=device)
         with pytest.raises(ValueError):
             norm_rope(big, big, None, None)
+
+
+@gpu
+@pytest.mark.parametrize("eps", [0.0, 1e-40])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_without_epsilon(dtype, eps):
+    """places of a tile and groups of lanes without a row add nothing to the gradients of the scales: rows of zeros have no norm there"""
+    from returnn_b200.ops.norm_rope import norm_rope, rope_frequencies
+
+    for n, hq, hk, d, rot in [(1, 1, 1, 64, 64), (7, 6, 1, 80, 80), (65, 3, 2, 128, 64), (7, 5, 5, 20, 10), (1, 2, 1, 8, 8), (300, 5, 3, 64, 0), (65, 7, 4, 256, 128)]:
+        for interleaved in (True, False):
+            q, k, _, wq, wk, pos = _inputs(n, hq, hk, d, dtype, "cuda", seed=n + d)
+            f = rope_frequencies(rot, device="cuda")[0] if rot else None
+            leaves = [x.detach().requires_grad_(True) for x in (q, k, wq, wk)]
+            out = norm_rope(leaves[0], leaves[1], pos, f, q_scale=leaves[2], k_scale=leaves[3], eps=eps, interleaved=interleaved)
+            g = torch.Generator().manual_seed(n)
+            dz = [torch.randn(o.shape, generator=g).cuda().to(dtype) for o in out]
+            got = torch.autograd.grad(out, leaves, dz)
+            wide = [x.detach().double().requires_grad_(True) for x in leaves]
+            exact = [_exact(wide[i], pos, f, wide[2 + i], eps, interleaved, 1.0)[0] for i in (0, 1)]
+            for i, (x, y) in enumerate(zip(got, torch.autograd.grad(exact, wide, [x.double() for x in dz]))):
+                rel = 2.0**-8 if x.dtype == torch.bfloat16 else 2.0**-17  # (as with an epsilon)
+                assert (x.double() - y).norm() <= rel * y.norm() + 1e-12, (n, hq, hk, d, rot, interleaved, i)
