@@ -15,7 +15,7 @@
 // What a warp keeps per query head are the running maximum, sum and output in registers.
 // bf16: products by warp-level matrix instructions (16 x 8 x 16). A decoding step has 1 to 32 rows per key head and is bound by memory: the
 // larger tensor-memory instructions have nothing to win (64 rows at least, keys would pass through descriptors) and the sixteen rows here are only half used:
-// rows 0..7 are 8 query heads with the weights rounded to bf16, rows 8..15 the same heads with what the rounding lost. Their sum weighs the
+// rows 0..7 are 8 query heads with the upper 16 bits of the weights, rows 8..15 the same heads with what is left of them in bf16. Their sum weighs the
 // values with 16 bits of mantissa at no further instruction; weights of 8 bits would add an error as large as the rounding of the result.
 // fp32: products by fused multiply-adds, a kernel for 1, 2, 4 and 8 heads of a unit (14 requests, 56340 tokens, D 128, 4 on each of 8 key heads: 88 us; with one kernel and the heads
 // counted at run time 169).
@@ -218,8 +218,13 @@ struct State<__nv_bfloat16, DP, 8> {
     for (int c = 0; c < 2; ++c) {
       const float p0 = exp2_of(x[2 * c], mn), p1 = exp2_of(x[2 * c + 1], mn);
       sum += p0 + p1;
-      hi[c] = pack2(p0, p1);
-      lo[c] = pack2(p0 - __uint_as_float(hi[c] << 16), p1 - __uint_as_float(hi[c] & 0xffff0000u));
+      // the upper half of a weight as it stands, and what is left, which is then above zero: an infinite value has to meet two weights of one sign (2^-126 of the values is
+      // added where nothing is left)
+      hi[c] = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
+      const __nv_bfloat162 rest = __floats2bfloat162_rn(p0 - __uint_as_float(hi[c] << 16), p1 - __uint_as_float(hi[c] & 0xffff0000u)),
+                           least = __halves2bfloat162(__ushort_as_bfloat16(0x0080), __ushort_as_bfloat16(0x0080));
+      const __nv_bfloat162 r = __hmax2(rest, least);
+      lo[c] = *reinterpret_cast<const uint32_t*>(&r);
     }
     l = l * f + sum;
     if (__any_sync(0xffffffffu, f != 1.f)) {

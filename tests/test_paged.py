@@ -367,3 +367,32 @@ def test_refusals(device):
     with pytest.raises(ValueError):
         release_pages(table, lens, lens, ring, rng, page_size=4)
     release_pages(table, lens, done, ring, rng, page_size=4)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_infinite_values(dtype):
+    """an infinite value with a weight above zero is in the output; infinities of both signs are no number; nothing else changes"""
+    from returnn_b200.ops.paged import paged_attention
+
+    lens = [1, 40, 2100, 300]
+    caches, table, g = _cache(4, 2, 64, 16, lens, dtype, 7)
+    kc, vc = caches.cuda().unbind(0)
+    q = torch.randn(4, 8, 64, generator=g).to("cuda", dtype)
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    plain = paged_attention(q, kc, vc, table, length)
+    assert plain.isfinite().all()
+    for places in ([0, 39, 2099, 17], [0, 0, 0, 0], [0, 20, 1024, 299]):
+        with_inf = vc.clone()
+        for i, t in enumerate(places):
+            page, at = table[i, t // 16], t % 16
+            with_inf[page, 0, at, 7], with_inf[page, 0, at, 8] = math.inf, -math.inf
+            if lens[i] > 1:
+                u = (t + 1) % lens[i]
+                with_inf[page, 0, at, 9], with_inf[table[i, u // 16], 0, u % 16, 9] = math.inf, -math.inf
+        got = paged_attention(q, kc, with_inf, table, length)
+        assert (got[:, :4, 7] == math.inf).all() and (got[:, :4, 8] == -math.inf).all() and got[1:, :4, 9].isnan().all()
+        same = torch.ones_like(got, dtype=torch.bool)
+        same[:, :4, 7:9] = False
+        same[1:, :4, 9] = False
+        assert torch.equal(got[same], plain[same])
