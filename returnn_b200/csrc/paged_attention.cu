@@ -830,10 +830,11 @@ static int group_of(int n, int units) {
   return g;
 }
 
-// bytes of workspace for n requests: cuts and parts of the CTAs
+// bytes of workspace for n requests: cuts and parts of the CTAs. None for shapes that are not computed
 RB_EXPORT long long rb200_paged_attention_workspace(int n, int heads, int kv_heads, int d, int bf16) {
+  if (n <= 0 || kv_heads <= 0 || heads < kv_heads) return 0;  // (no heads: no units to share them between)
   int uh;
-  const int units = kv_heads * units_of(heads / std::max(kv_heads, 1), bf16, &uh);
+  const int units = kv_heads * units_of(heads / kv_heads, bf16, &uh);
   return (long long)num_sms() * (16 + 2 * group_of(n, units) * uh * (d + 4) * 4);
 }
 

@@ -396,3 +396,30 @@ def test_attention_infinite_values(dtype):
         same[:, :4, 7:9] = False
         same[1:, :4, 9] = False
         assert torch.equal(got[same], plain[same])
+
+
+def test_workspace_without_heads():
+    """in a process of its own: a division by zero ends it"""
+    import os
+    import subprocess
+    import sys
+    from returnn_b200.ops import build
+
+    path = os.path.join(build._BUILD, "librb200.so")
+    if not os.path.exists(path):
+        pytest.skip("the kernels are not built")
+    code = ("import ctypes; f = ctypes.CDLL(%r).rb200_paged_attention_workspace; f.restype = ctypes.c_longlong; "
+            "print(f(1, 0, 1, 64, 1), f(0, 8, 2, 64, 1), f(3, 4, 0, 64, 0), f(3, 4, 2, 64, 0) > 0)" % path)
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and res.stdout.split() == ["0", "0", "0", "True"], (res.returncode, res.stdout, res.stderr)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_attention_without_heads_or_requests(device):
+    from returnn_b200.ops.paged import paged_attention
+
+    kc = torch.zeros(5, 2, 4, 16, device=device)
+    i32 = dict(dtype=torch.int32, device=device)
+    for n, heads in ((3, 0), (0, 4), (0, 0)):
+        out = paged_attention(torch.zeros(n, heads, 16, device=device), kc, kc, torch.zeros(n, 2, **i32), torch.ones(n, **i32))
+        assert out.shape == (n, heads, 16) and out.is_contiguous()
