@@ -537,7 +537,8 @@ struct RopeArgs {
 };
 // [..., heads, D] -> [N, heads, D] with unit stride over D
 Tensor token_rows(const Tensor& x) {
-  const Tensor y = x.dim() == 3 ? x : x.reshape({-1, x.size(-2), x.size(-1)});
+  // (the number of tokens by its axes: without heads the number of elements does not tell)
+  const Tensor y = x.dim() == 3 ? x : x.reshape({c10::multiply_integers(x.sizes().slice(0, x.dim() - 2)), x.size(-2), x.size(-1)});
   return y.stride(2) == 1 || y.size(2) == 1 ? y : y.contiguous();
 }
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }

@@ -283,3 +283,27 @@ def test_gradient_without_epsilon(dtype, eps):
             for i, (x, y) in enumerate(zip(got, torch.autograd.grad(exact, wide, [x.double() for x in dz]))):
                 rel = 2.0**-8 if x.dtype == torch.bfloat16 else 2.0**-17  # (as with an epsilon)
                 assert (x.double() - y).norm() <= rel * y.norm() + 1e-12, (n, hq, hk, d, rot, interleaved, i)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_no_heads_and_several_token_axes(device):
+    """results of no elements, and the other operand's as without them"""
+    from returnn_b200.ops.norm_rope import norm_rope, rope_frequencies
+
+    f, pos = rope_frequencies(64, device=device)[0], torch.arange(3, device=device)
+    w = [torch.ones(64, device=device, requires_grad=True) for _ in range(2)]
+    k = torch.randn(2, 3, 4, 64, generator=torch.Generator().manual_seed(1)).to(device).requires_grad_(True)
+    q = torch.empty(2, 3, 0, 64, device=device, requires_grad=True)
+    for scales in (dict(q_scale=w[0], k_scale=w[1]), {}):
+        oq, ok = norm_rope(q, k, pos, f, **scales)
+        same, alone = norm_rope(k, k, pos, f, **scales)
+        assert oq.shape == q.shape and torch.equal(ok, alone) and torch.equal(same, alone)
+        swapped = norm_rope(k, q, pos, f, **scales)
+        assert swapped[1].shape == q.shape and torch.equal(swapped[0], alone)
+        leaves = [q, k] + (w if scales else [])
+        got, want = torch.autograd.grad([oq, ok], leaves, [oq, ok.detach()]), torch.autograd.grad(alone, [k] + w[1:] * bool(scales), ok.detach())
+        assert got[0].shape == q.shape and torch.equal(got[1], want[0])
+        if scales:
+            assert not got[2].any() and torch.allclose(got[3], want[1], rtol=2.0**-20, atol=1e-6)
+        with torch.no_grad():
+            assert norm_rope(q, k, pos, f, **scales)[0].shape == q.shape
