@@ -766,14 +766,18 @@ RB_EXPORT int rb200_norm_rope_bwd(const void* dq, const void* dk, const void* q,
   if (bad_shape(a)) return RB_ERR_UNSUPPORTED;
   const bool norm = wq != nullptr;
   const int rows = hq + hk;
-  if (!norm && (n <= 0 || rows == 0)) return RB_OK;
+  if (n <= 0 || rows == 0) {  // sums of nothing; a launch for it would have as many groups as there are heads, more than places in `part`
+    const size_t bytes = (size_t)d * (w_bf16 ? 2 : 4);
+    if (norm && (cudaMemsetAsync(dwq, 0, bytes, stream) != cudaSuccess || cudaMemsetAsync(dwk, 0, bytes, stream) != cudaSuccess)) return rb_check_launch("norm_rope_bwd");
+    return RB_OK;
+  }
   a.inv_d = 1.f / d;
-  int64_t grid;  // (without any row one CTA leaves sums of zero)
+  int64_t grid;
   int gy = 1;
   if (fits(a, bf16, true, false)) {
     const int ctas = bf16 ? kBackCtasBf16 : kBackCtasF32;
     gy = tile_of(a, rows, kThreads / lanes_of(d), ctas, true);
-    grid = std::max<int64_t>(1, std::min<int64_t>((n + a.tokens - 1) / a.tokens, 148 * ctas / gy));
+    grid = std::min<int64_t>((n + a.tokens - 1) / a.tokens, 148 * ctas / gy);  // (gy: 148 * ctas at most, there is a tile)
     const size_t sums = norm ? (size_t)kThreads * 2 * 8 * sizeof(float) : 0;
     auto pick = [&](auto t) {
       return with_lanes(d, [&](auto l) {
@@ -786,7 +790,7 @@ RB_EXPORT int rb200_norm_rope_bwd(const void* dq, const void* dk, const void* q,
     auto kernel = bf16 ? pick(__nv_bfloat16()) : pick(float());
     rb_launch_pdl(kernel, dim3((unsigned)grid, (unsigned)gy), dim3(kThreads), smem_of(a) + sums, stream, a);
   } else {
-    grid = std::max<int64_t>(1, std::min<int64_t>((n * rows + kThreads / 32 - 1) / (kThreads / 32), kParts));
+    grid = std::min<int64_t>((n * rows + kThreads / 32 - 1) / (kThreads / 32), kParts);
     auto kernel = bf16 ? backward_any_kernel<__nv_bfloat16> : backward_any_kernel<float>;
     rb_launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
   }

@@ -307,3 +307,18 @@ def test_no_heads_and_several_token_axes(device):
             assert not got[2].any() and torch.allclose(got[3], want[1], rtol=2.0**-20, atol=1e-6)
         with torch.no_grad():
             assert norm_rope(q, k, pos, f, **scales)[0].shape == q.shape
+
+
+@gpu
+def test_gradient_without_tokens():
+    """scales of nothing have a gradient of zero, however many heads there are"""
+    from returnn_b200.ops.norm_rope import norm_rope, rope_frequencies
+
+    for hq, hk, d in ((5000, 9, 256), (4, 2, 64), (3, 3, 20), (0, 0, 64)):
+        q, k = (torch.empty(0, h, d, device="cuda", requires_grad=True) for h in (hq, hk))
+        for dtype in (torch.float32, torch.bfloat16):
+            w = [torch.ones(d, device="cuda", dtype=dtype, requires_grad=True) for _ in range(2)]
+            out = norm_rope(q, k, torch.empty(0, dtype=torch.int32, device="cuda"), rope_frequencies(d, device="cuda")[0], q_scale=w[0], k_scale=w[1])
+            got = torch.autograd.grad(out, [q, k] + w, [torch.empty_like(o) for o in out])
+            assert got[0].shape == q.shape and got[1].shape == k.shape
+            assert all(g.shape == (d,) and g.dtype == dtype and not g.any() for g in got[2:])
