@@ -500,6 +500,12 @@ bool wants_gradient(std::initializer_list<const Tensor*> tensors) {
     if (t && t->defined() && t->requires_grad()) return true;
   return false;
 }
+// a tangent of forward mode, which the kernels would drop: an autograd function raises an error for it, and so do the Python functions without a gradient
+bool has_tangent(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->_fw_grad(0).defined()) return true;
+  return false;
+}
 
 struct RopeArgs {
   Tensor positions, frequencies, wq, wk;  // undefined: none
@@ -604,16 +610,17 @@ struct NormRope : Function<NormRope> {
 };
 
 variable_list norm_rope(const Tensor& q, const Tensor& k, RopeArgs a) {
-  if (!a.fits(q, k)) return {};
+  if (!a.fits(q, k) || has_tangent({&a.frequencies})) return {};
   const c10::cuda::CUDAGuard guard(q.device());
-  if (wants_gradient({&q, &k, &a.wq, &a.wk})) return NormRope::apply(q, k, a.wq.defined() ? OptTensor(a.wq) : OptTensor(), a.wk.defined() ? OptTensor(a.wk) : OptTensor(), a);
+  if (wants_gradient({&q, &k, &a.wq, &a.wk}) || has_tangent({&q, &k, &a.wq, &a.wk}))
+    return NormRope::apply(q, k, a.wq.defined() ? OptTensor(a.wq) : OptTensor(), a.wk.defined() ? OptTensor(a.wk) : OptTensor(), a);
   auto [out_q, out_k] = norm_rope_forward(q, token_rows(q), k, token_rows(k), a, a.wq.defined() ? a.wq.contiguous() : a.wq, a.wk.defined() ? a.wk.contiguous() : a.wk);
   return {out_q, out_k};
 }
 
 Tensor norm_rope_to_cache(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cache_k, const Tensor& cache_v, const Tensor& slots, RopeArgs a) {
   if (q.dim() != 3 || !a.fits(q, k) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || v.device() != q.device() ||
-      wants_gradient({&q, &k, &v, &a.wq, &a.wk}))
+      wants_gradient({&q, &k, &v, &a.wq, &a.wk}) || has_tangent({&q, &k, &v, &a.wq, &a.wk, &a.frequencies, &cache_k, &cache_v}))
     return {};
   for (const Tensor* c : {&cache_k, &cache_v})
     if (c->dim() != 4 || c->size(1) != k.size(1) || c->size(3) != k.size(2) || c->sizes() != cache_k.sizes() || c->scalar_type() != q.scalar_type() ||
@@ -674,7 +681,9 @@ variable_list release_pages(const Tensor& table, const Tensor& lens, const Tenso
 }
 
 Tensor paged_attention(const Tensor& q, const Tensor& cache_k, const Tensor& cache_v, const Tensor& table, const Tensor& lens, double scale, const Tensor& status) {
-  if (!q.is_cuda() || q.dim() != 3 || cache_k.dim() != 4 || !bf16_or_fp32(q) || wants_gradient({&q, &cache_k, &cache_v})) return {};
+  if (!q.is_cuda() || q.dim() != 3 || cache_k.dim() != 4 || !bf16_or_fp32(q) || wants_gradient({&q, &cache_k, &cache_v}) ||
+      has_tangent({&q, &cache_k, &cache_v}))
+    return {};
   const int64_t n = q.size(0), heads = q.size(1), d = q.size(2), kv_heads = cache_k.size(1), unit = is_bf16(q) ? 8 : 4;
   if (cache_v.sizes() != cache_k.sizes() || cache_k.size(3) != d || kv_heads < 1 || heads % kv_heads || cache_k.size(2) < 1 || (q.stride(2) != 1 && d > 1)) return {};
   long long st[8] = {q.stride(0), q.stride(1)};
@@ -756,7 +765,7 @@ variable_list token_log_probs(const Tensor& x, const Tensor& targets, bool entro
       !targets.is_contiguous() || num_top < 0 || num_top > std::min<int64_t>(32, x.size(1)))
     return {};
   const c10::cuda::CUDAGuard guard(x.device());
-  if (!wants_gradient({&x})) {
+  if (!wants_gradient({&x}) && !has_tangent({&x})) {
     TokenScores r = token_log_probs_forward(x, targets, entropy, num_top, false);
     return {r.lp, r.entropy, r.top, r.labels};
   }

@@ -74,3 +74,9 @@ def of(tensor):
     if _lib._lib is None or _lib._env_data.get(b"RETURNN_B200_DISABLE_NATIVE", b"0") == b"1":
         return active() if _lib.use_native(tensor) else None
     return active()
+
+
+def has_tangent(*tensors) -> bool:
+    """:return: whether one of these has a tangent of forward mode, which a kernel without a derivative would drop"""
+    unpack = torch.autograd.forward_ad.unpack_dual
+    return any(t is not None and unpack(t).tangent is not None for t in tensors)

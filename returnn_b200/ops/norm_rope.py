@@ -97,6 +97,8 @@ def _check(q, k, positions, frequencies, q_scale, k_scale, what: str):
             raise ValueError("%s: frequencies must be fp32 [<= %i], got %s %s" % (what, d // 2, frequencies.dtype, tuple(frequencies.shape)))
         if positions.device != q.device or frequencies.device != q.device:
             raise ValueError("%s: positions on %s and frequencies on %s, q on %s" % (what, positions.device, frequencies.device, q.device))
+        if nodes.has_tangent(frequencies):
+            raise RuntimeError("%s: the frequencies have no derivative" % what)
     if (q_scale is None) != (k_scale is None):
         raise ValueError("%s: scales for both q and k, or for neither" % what)
     if q_scale is not None:
@@ -240,6 +242,8 @@ def norm_rope_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positi
         raise ValueError("%s: slots must be int32 [%i] on %s" % (what, q.shape[0], q.device))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, q_scale, k_scale)):
         raise RuntimeError("%s has no gradient: call it under torch.no_grad()" % what)
+    if nodes.has_tangent(q, k, v, q_scale, k_scale, k_cache, v_cache):
+        raise RuntimeError("%s has no derivative" % what)
     pages, page = k_cache.shape[0], k_cache.shape[2]
     if not _native_ok(q, q_scale, what):
         q, k = norm_rope_reference(q, k, positions, frequencies, q_scale=q_scale, k_scale=k_scale, eps=eps, interleaved=interleaved, amplitude=amplitude)

@@ -177,6 +177,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError("%s: lengths must be int32 [%i]" % (what, n))
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise RuntimeError("%s has no gradient: call it under torch.no_grad()" % what)
+    if nodes.has_tangent(q, k_cache, v_cache):
+        raise RuntimeError("%s has no derivative" % what)
     scale = float(d) ** -0.5 if scale is None else float(scale)
     if not (q.is_cuda and _lib.use_native(q)):
         return paged_attention_reference(q, k_cache, v_cache, block_table, lengths, scale=scale)

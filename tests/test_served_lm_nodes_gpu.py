@@ -83,3 +83,51 @@ def test_token_log_probs(monkeypatch, entropy, top):
     one = run()
     monkeypatch.setattr(nodes, "active", lambda: None)
     assert all(torch.equal(a, b) for a, b in zip(one, run()))
+
+
+def _rope_inputs():
+    from returnn_b200.ops.norm_rope import rope_frequencies
+
+    g = torch.Generator().manual_seed(0)
+    q, k = (torch.randn(5, h, 64, generator=g).cuda() for h in (3, 2))
+    w = [(torch.randn(64, generator=g) * 0.3 + 1.0).cuda() for _ in range(2)]
+    return q, k, w, rope_frequencies(32, device="cuda")[0], torch.arange(5, device="cuda")
+
+
+@gpu
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_function_transforms_are_refused(monkeypatch, python, grad_mode):
+    """torch.func and forward mode: an error, not a result without its derivative"""
+    from torch.autograd import forward_ad
+    from returnn_b200.ops import nodes
+    from returnn_b200.ops.norm_rope import norm_rope, norm_rope_to_cache
+    from returnn_b200.ops.paged import paged_attention
+    from returnn_b200.ops.token_log_probs import token_log_probs
+
+    if python:
+        monkeypatch.setattr(nodes, "active", lambda: None)
+    q, k, w, f, pos = _rope_inputs()
+    kc, vc = torch.zeros(2, 3, 2, 4, 64, device="cuda").unbind(0)
+    x, t = torch.randn(5, 40, device="cuda"), torch.arange(5, device="cuda")
+    slots, table, lens = (torch.zeros(*s, dtype=torch.int32, device="cuda") for s in ((5,), (5, 2), (5,)))
+    calls = [(lambda a: norm_rope(a, k, pos, f)[0], q), (lambda a: norm_rope(q, a, pos, f)[1], k), (lambda a: norm_rope(q, k, pos, f, q_scale=a, k_scale=w[1])[0], w[0]),
+             (lambda a: norm_rope(q, k, pos, f, q_scale=w[0], k_scale=a)[1], w[1]), (lambda a: norm_rope(q, k, pos, a)[0], f),
+             (lambda a: token_log_probs(a, t).log_probs, x), (lambda a: token_log_probs(a, t, entropy=True, num_top=2).entropy, x),
+             (lambda a: norm_rope_to_cache(a, k, k, pos, f, kc, vc, slots), q), (lambda a: norm_rope_to_cache(q, k, a, pos, f, kc, vc, slots), k),
+             (lambda a: norm_rope_to_cache(q, k, k, pos, f, a, vc, slots), kc),
+             (lambda a: paged_attention(a, kc, vc, table, lens), q[:, :2]), (lambda a: paged_attention(q[:, :2], kc, a, table, lens), vc)]
+    with torch.set_grad_enabled(grad_mode):
+        for i, (call, arg) in enumerate(calls):
+            with forward_ad.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+                call(forward_ad.make_dual(arg, torch.ones_like(arg)))
+            with pytest.raises(RuntimeError):
+                torch.func.vmap(lambda a: call(a))(arg[None])
+            if grad_mode:
+                with pytest.raises(RuntimeError):
+                    torch.func.grad(lambda a: call(a).sum())(arg)
+        with forward_ad.dual_level():  # a level without a tangent on these changes nothing
+            norm_rope(q, k, pos, f)
+            token_log_probs(x, t)
+            norm_rope_to_cache(q, k, k, pos, f, kc, vc, slots)
+            paged_attention(q[:, :2], kc, vc, table, lens)
