@@ -11,6 +11,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <atomic>
@@ -507,6 +509,19 @@ bool has_tangent(std::initializer_list<const Tensor*> tensors) {
   return false;
 }
 
+// Gradients `out` that have no derivatives of their own: where a graph of the backward pass is wanted and it depends on one of `from` that is part of a graph, to differentiate
+// them is an error, not a result that leaves them out
+variable_list first_order(const char* what, variable_list out, std::initializer_list<const Tensor*> from) {
+  if (!wants_gradient(from)) return out;
+  variable_list of;
+  for (const Tensor* t : from)
+    if (t->defined()) of.push_back(*t);
+  auto error = std::make_shared<torch::autograd::Error>(std::string(what) + " has no second derivative", torch::autograd::collect_next_edges(of));
+  for (const Tensor& t : out)
+    if (t.defined()) torch::autograd::set_history(t, error);
+  return out;
+}
+
 struct RopeArgs {
   Tensor positions, frequencies, wq, wk;  // undefined: none
   double eps, amp;
@@ -605,7 +620,7 @@ struct NormRope : Function<NormRope> {
                               (float)d.amp, stream()),
           "norm_rope_bwd");
     count(norm ? 2 : 1);
-    return {gq, gk, dwq, dwk, Tensor()};
+    return first_order("norm_rope", {gq, gk, dwq, dwk, Tensor()}, {&grads[0], &grads[1], &q3, &k3, &wq, &wk});
   }
 };
 
@@ -755,7 +770,7 @@ struct TokenLogProbs : Function<TokenLogProbs> {
                                     d_top.defined() ? d_top.stride(1) : 0, ptr(dx), x.size(0), (int)x.size(1), (int)num_top, is_bf16(x), stream()),
           "token_log_probs_bwd");
     count();
-    return {dx, Tensor(), Tensor(), Tensor()};
+    return first_order("token_log_probs", {dx, Tensor(), Tensor(), Tensor()}, {&d_lp, &d_entropy, &d_top, &x});
   }
 };
 // log probabilities, entropy, best, labels; undefined: not asked for

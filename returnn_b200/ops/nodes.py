@@ -80,3 +80,28 @@ def has_tangent(*tensors) -> bool:
     """:return: whether one of these has a tangent of forward mode, which a kernel without a derivative would drop"""
     unpack = torch.autograd.forward_ad.unpack_dual
     return any(t is not None and unpack(t).tangent is not None for t in tensors)
+
+
+class _FirstOrder(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, count, *tensors):
+        ctx.what = what
+        return tuple(t.detach() for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("%s has no second derivative" % ctx.what)
+
+
+def first_order(what: str, results, depend_on):
+    """
+    :param results: of the backward pass of a Python function that has no derivative of its own; None where there is no gradient
+    :param depend_on: tensors that went into them
+    :return: the results. Where a graph of the backward pass is wanted, to differentiate them is an error, not a result that leaves them out.
+    """
+    depend_on = [t for t in depend_on if t is not None and t.requires_grad]
+    if not depend_on or not torch.is_grad_enabled():
+        return tuple(results)
+    there = [t for t in results if t is not None]
+    marked = iter(_FirstOrder.apply(what, len(there), *there, *depend_on))
+    return tuple(None if t is None else next(marked) for t in results)

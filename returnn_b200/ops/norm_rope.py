@@ -179,7 +179,7 @@ class _NormRopeFn(torch.autograd.Function):
                           1 if wq is not None and wq.dtype == torch.bfloat16 else 0, 1 if interleaved else 0, eps, amplitude, _lib.stream_ptr()),
                        "norm_rope_bwd")
             _lib.count_launch(2 if wq is not None else 1)
-        return gq.view(ctx.shapes[0]), gk.view(ctx.shapes[1]), None, None, dwq, dwk, None, None, None
+        return nodes.first_order("norm_rope", (gq.view(ctx.shapes[0]), gk.view(ctx.shapes[1]), None, None, dwq, dwk, None, None, None), (dq, dk, q3, k3, wq, wk))
 
 
 def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tensor], frequencies: Optional[torch.Tensor], *,

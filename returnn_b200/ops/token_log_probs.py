@@ -74,7 +74,7 @@ class _TokenLogProbsFn(torch.autograd.Function):
                           _p(d_top), *(d_top.stride() if d_top is not None else (0, 0)), dx.data_ptr(), rows, v, ctx.num_top,
                           1 if x.dtype == torch.bfloat16 else 0, _lib.stream_ptr()), "token_log_probs_bwd")
             _lib.count_launch()
-        return dx, None, None, None
+        return nodes.first_order("token_log_probs", (dx, None, None, None), (d_lp, d_ent, d_top, x))
 
 
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, *, entropy: bool = False, num_top: int = 0) -> TokenLogProbs:

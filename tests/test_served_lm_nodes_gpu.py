@@ -131,3 +131,32 @@ def test_function_transforms_are_refused(monkeypatch, python, grad_mode):
             token_log_probs(x, t)
             norm_rope_to_cache(q, k, k, pos, f, kc, vc, slots)
             paged_attention(q[:, :2], kc, vc, table, lens)
+
+
+@gpu
+@pytest.mark.parametrize("python", [False, True])
+def test_second_derivatives_are_refused(monkeypatch, python):
+    """an error where a gradient is differentiated through these operators, not a result that leaves them out"""
+    from returnn_b200.ops import nodes
+    from returnn_b200.ops.norm_rope import norm_rope
+    from returnn_b200.ops.token_log_probs import token_log_probs
+
+    if python:
+        monkeypatch.setattr(nodes, "active", lambda: None)
+    q, k, w, f, pos = _rope_inputs()
+    q, w = q.requires_grad_(True), [x.requires_grad_(True) for x in w]
+    c = torch.randn(q.shape, device="cuda")
+    x = torch.randn(5, 40, device="cuda", requires_grad=True)
+    t = torch.arange(5, device="cuda")
+    for loss, leaf in (((norm_rope(q, k, pos, f, q_scale=w[0], k_scale=w[1])[0] * c).sum(), q), ((norm_rope(q, k, pos, f, q_scale=w[0], k_scale=w[1])[0] * c).sum(), w[0]),
+                       (norm_rope(q, k, pos, f)[0].square().sum(), q), (token_log_probs(x, t).log_probs.sum(), x),
+                       (token_log_probs(x, t, entropy=True, num_top=2).top_log_probs.sum(), x)):
+        (first,) = torch.autograd.grad(loss, leaf, create_graph=True, retain_graph=True)
+        (again,) = torch.autograd.grad(loss, leaf)
+        assert torch.equal(first, again)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad((first.square().sum() + leaf.square().sum()), leaf)
+    # a rotation alone is linear: its gradient does not depend on what was rotated
+    (first,) = torch.autograd.grad((norm_rope(q, k, pos, f)[0] * c).sum(), q, create_graph=True)
+    (second,) = torch.autograd.grad(first.sum() + q.square().sum(), q)
+    assert torch.equal(second, 2 * q)
