@@ -535,7 +535,7 @@ struct RopeArgs {
     for (int64_t i = 0; i + 2 < n; ++i)
       if (q.size(i) != k.size(i)) return false;
     if (frequencies.defined()) {
-      if (!positions.defined() || (positions.scalar_type() != at::kInt && positions.scalar_type() != at::kLong) || positions.device() != q.device() ||
+      if (wants_gradient({&frequencies}) || has_tangent({&frequencies}) || !positions.defined() || (positions.scalar_type() != at::kInt && positions.scalar_type() != at::kLong) || positions.device() != q.device() ||
           frequencies.device() != q.device() || frequencies.dim() != 1 || frequencies.scalar_type() != at::kFloat || 2 * frequencies.size(0) > d || positions.dim() > n - 2)
         return false;
       for (int64_t i = 0; i < positions.dim(); ++i)
@@ -625,7 +625,7 @@ struct NormRope : Function<NormRope> {
 };
 
 variable_list norm_rope(const Tensor& q, const Tensor& k, RopeArgs a) {
-  if (!a.fits(q, k) || has_tangent({&a.frequencies})) return {};
+  if (!a.fits(q, k)) return {};
   const c10::cuda::CUDAGuard guard(q.device());
   if (wants_gradient({&q, &k, &a.wq, &a.wk}) || has_tangent({&q, &k, &a.wq, &a.wk}))
     return NormRope::apply(q, k, a.wq.defined() ? OptTensor(a.wq) : OptTensor(), a.wk.defined() ? OptTensor(a.wk) : OptTensor(), a);
@@ -635,7 +635,7 @@ variable_list norm_rope(const Tensor& q, const Tensor& k, RopeArgs a) {
 
 Tensor norm_rope_to_cache(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cache_k, const Tensor& cache_v, const Tensor& slots, RopeArgs a) {
   if (q.dim() != 3 || !a.fits(q, k) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || v.device() != q.device() ||
-      wants_gradient({&q, &k, &v, &a.wq, &a.wk}) || has_tangent({&q, &k, &v, &a.wq, &a.wk, &a.frequencies, &cache_k, &cache_v}))
+      wants_gradient({&q, &k, &v, &a.wq, &a.wk}) || has_tangent({&q, &k, &v, &a.wq, &a.wk, &cache_k, &cache_v}))
     return {};
   for (const Tensor* c : {&cache_k, &cache_v})
     if (c->dim() != 4 || c->size(1) != k.size(1) || c->size(3) != k.size(2) || c->sizes() != cache_k.sizes() || c->scalar_type() != q.scalar_type() ||

@@ -97,8 +97,8 @@ def _check(q, k, positions, frequencies, q_scale, k_scale, what: str):
             raise ValueError("%s: frequencies must be fp32 [<= %i], got %s %s" % (what, d // 2, frequencies.dtype, tuple(frequencies.shape)))
         if positions.device != q.device or frequencies.device != q.device:
             raise ValueError("%s: positions on %s and frequencies on %s, q on %s" % (what, positions.device, frequencies.device, q.device))
-        if nodes.has_tangent(frequencies):
-            raise RuntimeError("%s: the frequencies have no derivative" % what)
+        if (torch.is_grad_enabled() and frequencies.requires_grad) or nodes.has_tangent(frequencies):
+            raise RuntimeError("%s: there is no gradient of the frequencies: detach them" % what)
     if (q_scale is None) != (k_scale is None):
         raise ValueError("%s: scales for both q and k, or for neither" % what)
     if q_scale is not None:
@@ -186,7 +186,8 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tensor
               q_scale: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = True,
               amplitude: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """
-    Norm per head and rotation of queries and keys (see the module docstring); differentiable in ``q``, ``k`` and the scales.
+    Norm per head and rotation of queries and keys (see the module docstring); differentiable in ``q``, ``k`` and the scales, once. Frequencies that require a gradient are
+    refused.
 
     :param q: [..., heads, D] bf16 or fp32; any strides with unit stride over D (slices of a fused projection are read in place)
     :param k: [..., key heads, D] over the same tokens

@@ -322,3 +322,21 @@ def test_gradient_without_tokens():
             got = torch.autograd.grad(out, [q, k] + w, [torch.empty_like(o) for o in out])
             assert got[0].shape == q.shape and got[1].shape == k.shape
             assert all(g.shape == (d,) and g.dtype == dtype and not g.any() for g in got[2:])
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_frequencies_have_no_gradient(device):
+    from returnn_b200.ops.norm_rope import norm_rope, norm_rope_to_cache, rope_frequencies
+
+    q, k, v, _, _, pos = _inputs(6, 4, 2, 16, torch.float32, device)
+    f = rope_frequencies(16, device=device)[0].requires_grad_(True)
+    kc, vc = torch.zeros(2, 4, 2, 3, 16, device=device).unbind(0)
+    slots = torch.arange(6, dtype=torch.int32, device=device)
+    with pytest.raises(RuntimeError, match="frequencies"):
+        norm_rope(q, k, pos, f)
+    with pytest.raises(RuntimeError):
+        norm_rope_to_cache(q, k, v, pos, f, kc, vc, slots)
+    with torch.no_grad():
+        want = norm_rope(q, k, pos, f.detach())
+        assert all(torch.equal(a, b) for a, b in zip(norm_rope(q, k, pos, f), want))
+        assert torch.equal(norm_rope_to_cache(q, k, v, pos, f, kc, vc, slots), want[0])
