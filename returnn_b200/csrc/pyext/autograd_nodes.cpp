@@ -502,6 +502,11 @@ bool wants_gradient(std::initializer_list<const Tensor*> tensors) {
     if (t && t->defined() && t->requires_grad()) return true;
   return false;
 }
+// a kernel changed what is in these: autograd compares the number of changes with that of when it saved a tensor
+void written(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 // a tangent of forward mode, which the kernels would drop: an autograd function raises an error for it, and so do the Python functions without a gradient
 bool has_tangent(std::initializer_list<const Tensor*> tensors) {
   for (const Tensor* t : tensors)
@@ -635,7 +640,7 @@ variable_list norm_rope(const Tensor& q, const Tensor& k, RopeArgs a) {
 
 Tensor norm_rope_to_cache(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cache_k, const Tensor& cache_v, const Tensor& slots, RopeArgs a) {
   if (q.dim() != 3 || !a.fits(q, k) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || v.device() != q.device() ||
-      wants_gradient({&q, &k, &v, &a.wq, &a.wk}) || has_tangent({&q, &k, &v, &a.wq, &a.wk, &cache_k, &cache_v}))
+      wants_gradient({&q, &k, &v, &a.wq, &a.wk, &cache_k, &cache_v}) || has_tangent({&q, &k, &v, &a.wq, &a.wk, &cache_k, &cache_v}))
     return {};
   for (const Tensor* c : {&cache_k, &cache_v})
     if (c->dim() != 4 || c->size(1) != k.size(1) || c->size(3) != k.size(2) || c->sizes() != cache_k.sizes() || c->scalar_type() != q.scalar_type() ||
@@ -653,6 +658,7 @@ Tensor norm_rope_to_cache(const Tensor& q, const Tensor& k, const Tensor& v, con
                               cache_k.size(0) * cache_k.size(2), is_bf16(q), a.is64(), a.w_bf16(), a.interleaved, (float)a.eps, (float)a.amp, stream()),
         "norm_rope_to_cache");
   count();
+  written({&cache_k, &cache_v});
   return out;
 }
 
@@ -680,6 +686,7 @@ variable_list append_tokens(const Tensor& table, const Tensor& lens, const Tenso
                            ptr<long long>(new_range), ptr(granted), stream()),
         "append_tokens");
   count();
+  written({&table});
   return {slots, positions, requests, offsets, new_lens, new_range, granted};
 }
 variable_list release_pages(const Tensor& table, const Tensor& lens, const Tensor& done, const Tensor& ring, const Tensor& range, int64_t page) {
@@ -692,6 +699,7 @@ variable_list release_pages(const Tensor& table, const Tensor& lens, const Tenso
                             (int)page, ptr<int>(new_lens), ptr<long long>(new_range), stream()),
         "release_pages");
   count();
+  written({&ring});
   return {new_lens, new_range};
 }
 

@@ -105,3 +105,10 @@ def first_order(what: str, results, depend_on):
     there = [t for t in results if t is not None]
     marked = iter(_FirstOrder.apply(what, len(there), *there, *depend_on))
     return tuple(None if t is None else next(marked) for t in results)
+
+
+def written(*tensors):
+    """a kernel changed what is in these: autograd compares the number of changes with that of when it saved a tensor"""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)

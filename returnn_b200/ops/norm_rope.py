@@ -241,7 +241,7 @@ def norm_rope_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positi
             raise ValueError("%s: caches need unit stride over the features" % what)
     if slots.shape != q.shape[:1] or slots.dtype != torch.int32 or slots.device != q.device:
         raise ValueError("%s: slots must be int32 [%i] on %s" % (what, q.shape[0], q.device))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, q_scale, k_scale)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, q_scale, k_scale, k_cache, v_cache)):
         raise RuntimeError("%s has no gradient: call it under torch.no_grad()" % what)
     if nodes.has_tangent(q, k, v, q_scale, k_scale, k_cache, v_cache):
         raise RuntimeError("%s has no derivative" % what)
@@ -271,6 +271,7 @@ def norm_rope_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positi
                       1 if wq is not None and wq.dtype == torch.bfloat16 else 0, 1 if interleaved else 0, float(eps), float(amplitude), _lib.stream_ptr()),
                    "norm_rope_to_cache")
         _lib.count_launch()
+        nodes.written(k_cache, v_cache)
     return out_q
 
 

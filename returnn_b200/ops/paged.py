@@ -108,6 +108,7 @@ def append_tokens(block_table: torch.Tensor, lengths: torch.Tensor, counts: torc
                       free_range.data_ptr(), page_size, max_tokens, slots.data_ptr(), positions.data_ptr(), requests.data_ptr(), offsets.data_ptr(),
                       new_lengths.data_ptr(), new_range.data_ptr(), granted.data_ptr(), _lib.stream_ptr()), what)
         _lib.count_launch()
+        nodes.written(block_table)
     return AppendedTokens(slots, positions, requests, offsets, new_lengths, new_range, granted)
 
 
@@ -138,6 +139,7 @@ def release_pages(block_table: torch.Tensor, lengths: torch.Tensor, finished: to
         _lib.check(fn(block_table.data_ptr(), block_table.stride(0), blocks, lengths.data_ptr(), finished.data_ptr(), n, free_pages.data_ptr(), free_pages.shape[0],
                       free_range.data_ptr(), page_size, new_lengths.data_ptr(), new_range.data_ptr(), _lib.stream_ptr()), what)
         _lib.count_launch()
+        nodes.written(free_pages)
     return ReleasedPages(new_lengths, new_range)
 
 

@@ -340,3 +340,30 @@ def test_frequencies_have_no_gradient(device):
         want = norm_rope(q, k, pos, f.detach())
         assert all(torch.equal(a, b) for a, b in zip(norm_rope(q, k, pos, f), want))
         assert torch.equal(norm_rope_to_cache(q, k, v, pos, f, kc, vc, slots), want[0])
+
+
+@pytest.mark.parametrize("device,python", [("cpu", False), pytest.param("cuda", False, marks=gpu), pytest.param("cuda", True, marks=gpu)])
+def test_caches_written_in_place(monkeypatch, device, python):
+    """autograd learns of the write: a cache that a graph still needs is noticed, one that requires a gradient refused"""
+    from returnn_b200.ops import nodes
+    from returnn_b200.ops.norm_rope import norm_rope_to_cache, rope_frequencies
+
+    if python:
+        monkeypatch.setattr(nodes, "active", lambda: None)
+    q, k, v, _, _, pos = _inputs(6, 4, 2, 16, torch.float32, device)
+    f = rope_frequencies(16, device=device)[0]
+    kc, vc = (torch.zeros(4, 2, 3, 16, device=device) for _ in range(2))
+    slots = torch.arange(6, dtype=torch.int32, device=device)
+    x = torch.ones_like(kc).requires_grad_(True)
+    loss = (x * kc).sum() + (x * vc).sum()
+    norm_rope_to_cache(q, k, v, pos, f, kc, vc, slots)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    for caches in ((kc.clone().requires_grad_(True), vc), (kc, vc.clone().requires_grad_(True)), (kc, vc * x)):
+        with pytest.raises(RuntimeError):
+            norm_rope_to_cache(q, k, v, pos, f, *caches, slots)
+    with torch.inference_mode():
+        inner = torch.zeros(2, 4, 2, 3, 16, device=device)
+        norm_rope_to_cache(q, k, v, pos, f, inner[0], inner[1], slots)
+    norm_rope_to_cache(q, k, v, pos, f, kc, vc, slots)
+    assert torch.equal(inner[0], kc) and torch.equal(inner[1], vc)

@@ -423,3 +423,23 @@ def test_attention_without_heads_or_requests(device):
     for n, heads in ((3, 0), (0, 4), (0, 0)):
         out = paged_attention(torch.zeros(n, heads, 16, device=device), kc, kc, torch.zeros(n, 2, **i32), torch.ones(n, **i32))
         assert out.shape == (n, heads, 16) and out.is_contiguous()
+
+
+@pytest.mark.parametrize("device,python", [("cpu", False), pytest.param("cuda", False, marks=gpu), pytest.param("cuda", True, marks=gpu)])
+def test_tables_written_in_place(monkeypatch, device, python):
+    """autograd learns of the writes: a table or a ring that a graph still needs as an index is noticed"""
+    from returnn_b200.ops import nodes
+    from returnn_b200.ops.paged import append_tokens, release_pages
+
+    if python:
+        monkeypatch.setattr(nodes, "active", lambda: None)
+    i32 = dict(dtype=torch.int32, device=device)
+    table, ring, rng = torch.zeros(2, 3, **i32), torch.arange(6, **i32), torch.tensor([0, 6], device=device)
+    x = torch.randn(6, 4, device=device, requires_grad=True)
+    by_table, by_ring = x.index_select(0, table.view(-1)).sum(), x.index_select(0, ring).sum()
+    r = append_tokens(table, torch.zeros(2, **i32), torch.tensor([5, 4], **i32), ring, rng, page_size=4, max_tokens=9)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        by_table.backward()
+    release_pages(table, r.lengths, torch.ones(2, dtype=torch.bool, device=device), ring, r.free_range, page_size=4)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        by_ring.backward()
