@@ -670,7 +670,8 @@ bool pages_fit(const Tensor& table, const Tensor& lens, const Tensor& per, at::S
          ring.device() == table.device() && range.dim() == 1 && range.size(0) == 2 && range.scalar_type() == at::kLong && range.device() == table.device() && range.is_contiguous();
 }
 variable_list append_tokens(const Tensor& table, const Tensor& lens, const Tensor& counts, const Tensor& ring, const Tensor& range, int64_t page, int64_t max_tokens) {
-  if (!pages_fit(table, lens, counts, at::kInt, ring, range, page) || max_tokens < 0 || page > INT_MAX) return {};
+  if (!pages_fit(table, lens, counts, at::kInt, ring, range, page) || max_tokens < 0 || page > INT_MAX || ring.numel() > (1LL << 31) / page)
+    return {};
   const c10::cuda::CUDAGuard guard(table.device());
   const int64_t n = table.size(0);
   Tensor slots, positions, requests, offsets, new_lens, new_range, granted;

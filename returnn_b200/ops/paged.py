@@ -78,7 +78,7 @@ def append_tokens(block_table: torch.Tensor, lengths: torch.Tensor, counts: torc
     :param block_table: [requests, blocks] int32
     :param lengths: [requests] int32 tokens so far
     :param counts: [requests] int32 new tokens, 0 where there are none
-    :param free_pages: [pages] int32, the ring
+    :param free_pages: [pages] int32, the ring; pages times page size at most 2^31
     :param free_range: [2] int64
     :param max_tokens: room for new tokens, at least ``counts.sum()`` (tokens beyond it are left out of the lists, not of the lengths)
     """
@@ -91,6 +91,8 @@ def append_tokens(block_table: torch.Tensor, lengths: torch.Tensor, counts: torc
     _check_table(what, block_table, lengths, counts, torch.int32, free_pages, free_range, page_size)
     if max_tokens < 0:
         raise ValueError("%s: max_tokens %r" % (what, max_tokens))
+    if free_pages.shape[0] * page_size > 2**31:
+        raise ValueError("%s: %i pages of %i tokens, slots have 31 bits" % (what, free_pages.shape[0], page_size))
     if not (block_table.is_cuda and _lib.use_native(block_table)):
         return append_tokens_reference(block_table, lengths, counts, free_pages, free_range, page_size=page_size, max_tokens=max_tokens)
     with torch.cuda.device_of(block_table):

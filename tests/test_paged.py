@@ -443,3 +443,15 @@ def test_tables_written_in_place(monkeypatch, device, python):
     release_pages(table, r.lengths, torch.ones(2, dtype=torch.bool, device=device), ring, r.free_range, page_size=4)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         by_ring.backward()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_slots_beyond_32_bits_are_refused(device):
+    from returnn_b200.ops.paged import append_tokens
+
+    i32 = dict(dtype=torch.int32, device=device)
+    lens, counts, rng = torch.zeros(1, **i32), torch.ones(1, **i32), torch.tensor([0, 3], device=device)
+    with pytest.raises(ValueError):
+        append_tokens(torch.full((1, 2), -1, **i32), lens, counts, torch.tensor([2, 1, 0], **i32), rng, page_size=2**30, max_tokens=1)
+    r = append_tokens(torch.full((1, 2), -1, **i32), lens, counts, torch.tensor([1, 0], **i32), rng - 1, page_size=2**30, max_tokens=1)
+    assert r.slots.tolist() == [0] and r.granted.tolist() == [True]
