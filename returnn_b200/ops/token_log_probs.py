@@ -3,7 +3,7 @@ Log probabilities of given tokens, with the entropy of their distributions and t
 (``csrc/token_log_probs.cu``). What scoring, rescoring and sequence training with a language model read off its output layer.
 
 With ``p = softmax(x)`` per row: ``log_probs = log p[target]``, ``entropy = -sum p log p``, ``top_labels`` the ``num_top`` largest logits (the lowest
-label first among equal ones, NaN counts as the largest) and ``top_log_probs`` their ``log p``. Sums are taken in 32 bits.
+label first among equal ones, NaN counts as the largest, numbers below 2^-126 in size as 0) and ``top_log_probs`` their ``log p``. Sums are taken in 32 bits.
 
 A target outside ``0 .. V - 1`` (a padded position) has log probability 0 without a gradient. A label of logit -inf has probability 0. A row in which no label
 has a probability has entropy 0, log probabilities -inf and no gradient.
@@ -119,6 +119,9 @@ def token_log_probs_reference(logits, targets, *, entropy=False, num_top=0):
         finite = torch.where(lp == -math.inf, 0.0, lp)
         res = res._replace(entropy=-(lp.exp() * finite).sum(dim=-1))
     if num_top:
-        labels = torch.sort(torch.where(x.isnan(), math.nan, x).detach(), dim=-1, descending=True, stable=True)[1][:, :num_top]
+        order = torch.where(x.isnan(), math.nan, x).detach()
+        if x.dtype == torch.float32:
+            order = torch.where(order.abs() < torch.finfo(torch.float32).tiny, 0.0, order)
+        labels = torch.sort(order, dim=-1, descending=True, stable=True)[1][:, :num_top]
         res = res._replace(top_log_probs=lp.gather(-1, labels), top_labels=labels.to(torch.int32))
     return res

@@ -255,3 +255,18 @@ def test_refusals_and_empty(device):
             token_log_probs(x.half(), t)
     r = token_log_probs(x[:0], t[:0], entropy=True, num_top=3)
     assert r.log_probs.shape == r.entropy.shape == (0,) and r.top_labels.shape == (0, 3)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_logits_below_the_normal_numbers_are_zeros(dtype, device):
+    """their differences do not show in 32 bits of a log probability: they are equal, the lowest label comes first, on either device"""
+    from returnn_b200.ops.token_log_probs import token_log_probs
+
+    for v in (9, 300, 20_000):
+        x = (torch.arange(v, dtype=torch.float32) % 100 - 50.0).mul_(2.0**-133).to(dtype)[None].repeat(3, 1)
+        x[1, v // 2], x[1, v - 1] = 2.0**-126, -(2.0**-126)  # the smallest that count
+        x[2] = -1.0
+        x[2, v - 2], x[2, 1] = 2.0**-130, -(2.0**-130)
+        r = token_log_probs(x.to(device), torch.zeros(3, dtype=torch.int64, device=device), num_top=5)
+        assert r.top_labels.tolist() == [[0, 1, 2, 3, 4], [v // 2] + [i for i in range(6) if i != v // 2][:4], [1, v - 2, 0] + [i for i in range(2, 6) if i != v - 2][:2]]
