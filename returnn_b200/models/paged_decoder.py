@@ -149,6 +149,12 @@ class PagedDecoder:
 
     # ---- requests
 
+    def _check_prompt(self, labels: Sequence[int]):
+        if not 0 < len(labels) <= self.max_len:
+            raise ValueError("paged decoder: a prompt of %i labels (1 to %i)" % (len(labels), self.max_len))
+        if not (0 <= min(labels) and max(labels) < self.emb.shape[0]):  # (here, not by the lookup on the device)
+            raise ValueError("paged decoder: labels %i to %i, the vocabulary has %i" % (min(labels), max(labels), self.emb.shape[0]))
+
     def add(self, rows: Sequence[int], prompts: Sequence[Sequence[int]]) -> torch.Tensor:
         """
         New requests in empty rows: their prompts take pages and run through the layers.
@@ -159,8 +165,7 @@ class PagedDecoder:
             order = sorted(range(len(rows)), key=lambda i: rows[i])  # (tokens of a call lie in the order of the rows)
             counts = torch.zeros(self.rows, dtype=torch.int32)
             for i in order:
-                if not 0 < len(prompts[i]) <= self.max_len:
-                    raise ValueError("paged decoder: a prompt of %i labels (1 to %i)" % (len(prompts[i]), self.max_len))
+                self._check_prompt(prompts[i])
                 counts[rows[i]] = len(prompts[i])
             labels = torch.tensor([t for i in order for t in prompts[i]], dtype=torch.int64).to(self.device)
             total = len(labels)
