@@ -163,9 +163,10 @@ class PagedDecoder:
         """
         with torch.no_grad(), torch.autocast(self.device.type, enabled=False):
             order = sorted(range(len(rows)), key=lambda i: rows[i])  # (tokens of a call lie in the order of the rows)
+            for prompt in prompts:
+                self._check_prompt(prompt)
             counts = torch.zeros(self.rows, dtype=torch.int32)
             for i in order:
-                self._check_prompt(prompts[i])
                 counts[rows[i]] = len(prompts[i])
             labels = torch.tensor([t for i in order for t in prompts[i]], dtype=torch.int64).to(self.device)
             total = len(labels)
@@ -186,9 +187,13 @@ class PagedDecoder:
                 out = _att.sdpa(q, k, v, kv_lens=lens[:, None].expand(n, lay["h"]), scale=lay["d"] ** -0.5, causal=True)
                 return out.transpose(1, 2).reshape(n * longest, -1).index_select(0, place)
 
-            x = self._embed(labels, new.positions)
-            for lay in self.layers:
-                x = self._layer(lay, x, new, attend)
+            try:
+                x = self._embed(labels, new.positions)
+                for lay in self.layers:
+                    x = self._layer(lay, x, new, attend)
+            except BaseException:
+                self.end(rows)
+                raise
             return x[self._unsorted(order, [len(p) for p in prompts])] if order != list(range(len(rows))) else x
 
     def _unsorted(self, order, lens) -> torch.Tensor:
@@ -255,14 +260,15 @@ class PagedDecoder:
             part = texts[at: at + self.rows]
             rows = list(range(len(part)))
             x = self.add(rows, part)
-            lens = self.lengths[: len(part)].tolist()
-            if any(have != len(t) for have, t in zip(lens, part)):
+            try:
+                lens = self.lengths[: len(part)].tolist()
+                if any(have != len(t) for have, t in zip(lens, part)):
+                    raise RuntimeError("paged decoder: no room for %i texts in %i pages" % (len(part), self.num_pages))
+                targets = torch.tensor([y for t in part for y in list(t[1:]) + [-1]], dtype=torch.int32).to(self.device)
+                with torch.no_grad():
+                    r = token_log_probs(self._logits(x), targets, entropy=True, num_top=num_top)
+            finally:
                 self.end(rows)
-                raise RuntimeError("paged decoder: no room for %i texts in %i pages" % (len(part), self.num_pages))
-            targets = torch.tensor([y for t in part for y in list(t[1:]) + [-1]], dtype=torch.int32).to(self.device)
-            with torch.no_grad():
-                r = token_log_probs(self._logits(x), targets, entropy=True, num_top=num_top)
-            self.end(rows)
             first = 0
             for t in part:
                 cut = slice(first, first + len(t) - 1)
@@ -275,6 +281,8 @@ class PagedDecoder:
         The best label after each prompt, and so on until ``eos`` or ``max_new`` labels or the longest length. Prompts beyond the number of rows, or without pages at the moment, wait until
         others end. One that does not fit the pool alone is an error.
         """
+        for prompt in prompts:
+            self._check_prompt(prompt)
         out = [GeneratedText([], []) for _ in prompts]
         waiting = list(range(len(prompts)))
         running = {}  # row -> prompt
@@ -286,50 +294,58 @@ class PagedDecoder:
             out[i].log_probs.append(log_prob)
             return label != eos and len(out[i].labels) < max_new and len(prompts[i]) + len(out[i].labels) < self.max_len
 
-        while waiting or running:
-            free = [r for r in range(self.rows) if r not in running]
-            if waiting and free:
-                rows = free[: len(waiting)]
-                batch = waiting[: len(rows)]
-                x = self.add(rows, [prompts[i] for i in batch])
-                have = self.lengths.tolist()
-                ends = torch.tensor([len(prompts[i]) for i in batch]).cumsum(0) - 1
-                with torch.no_grad():
-                    best = token_log_probs(self._logits(x[ends.to(self.device)]), self._ignored[: len(batch)], num_top=1)
-                over = []
-                for r, i, label, lp in zip(rows, batch, best.top_labels[:, 0].tolist(), best.top_log_probs[:, 0].tolist()):
-                    if not have[r]:  # the pool was empty: again later
-                        continue
-                    waiting.remove(i)
-                    if max_new > 0 and take(i, label, lp):
-                        running[r], last[r] = i, label
+        held = set()  # rows that may have pages
+        try:
+            while waiting or running:
+                free = [r for r in range(self.rows) if r not in running]
+                if waiting and free:
+                    rows = free[: len(waiting)]
+                    batch = waiting[: len(rows)]
+                    held.update(rows)
+                    x = self.add(rows, [prompts[i] for i in batch])
+                    have = self.lengths.tolist()
+                    ends = torch.tensor([len(prompts[i]) for i in batch]).cumsum(0) - 1
+                    with torch.no_grad():
+                        best = token_log_probs(self._logits(x[ends.to(self.device)]), self._ignored[: len(batch)], num_top=1)
+                    over = []
+                    for r, i, label, lp in zip(rows, batch, best.top_labels[:, 0].tolist(), best.top_log_probs[:, 0].tolist()):
+                        if not have[r]:  # the pool was empty: again later
+                            continue
+                        waiting.remove(i)
+                        if max_new > 0 and take(i, label, lp):
+                            running[r], last[r] = i, label
+                        else:
+                            over.append(r)
+                    if over:
+                        self.end(over)
+                        held.difference_update(over)
+                    elif not running:
+                        raise RuntimeError("paged decoder: prompts of %s labels do not fit %i pages" % ([len(prompts[i]) for i in batch], self.num_pages))
+                if not running:
+                    continue
+                active.zero_()
+                active[list(running)] = 1
+                self._active.copy_(active)
+                self._last.copy_(last)
+                labels, log_probs, requests, granted = self.step(use_graph=use_graph)
+                over, stuck = [], []
+                for r, label, lp, ok in zip(requests.tolist(), labels.tolist(), log_probs.tolist(), granted[requests.clamp(min=0).long()].tolist()):
+                    if r < 0:
+                        break
+                    if not ok:  # no page was left for it in this step; it goes on when another ends
+                        stuck.append(r)
+                    elif take(running[r], label, lp):
+                        last[r] = label
                     else:
                         over.append(r)
+                if stuck and len(stuck) == len(running):
+                    raise RuntimeError("paged decoder: %i running requests and no free page of %i" % (len(stuck), self.num_pages))
+                for r in over:
+                    del running[r]
                 if over:
                     self.end(over)
-                elif not running:
-                    raise RuntimeError("paged decoder: prompts of %s labels do not fit %i pages" % ([len(prompts[i]) for i in batch], self.num_pages))
-            if not running:
-                continue
-            active.zero_()
-            active[list(running)] = 1
-            self._active.copy_(active)
-            self._last.copy_(last)
-            labels, log_probs, requests, granted = self.step(use_graph=use_graph)
-            over, stuck = [], []
-            for r, label, lp, ok in zip(requests.tolist(), labels.tolist(), log_probs.tolist(), granted[requests.clamp(min=0).long()].tolist()):
-                if r < 0:
-                    break
-                if not ok:  # no page was left for it in this step; it goes on when another ends
-                    stuck.append(r)
-                elif take(running[r], label, lp):
-                    last[r] = label
-                else:
-                    over.append(r)
-            if stuck and len(stuck) == len(running):
-                raise RuntimeError("paged decoder: %i running requests and no free page of %i" % (len(stuck), self.num_pages))
-            for r in over:
-                del running[r]
-            if over:
-                self.end(over)
+                    held.difference_update(over)
+        finally:
+            if held:
+                self.end(sorted(held))
         return out

@@ -29,3 +29,40 @@ def test_labels_outside_the_vocabulary_are_refused():
                 call()
             assert _is_empty(paged)
     assert len(paged.score([[60, 0]])[0].log_probs) == 1
+
+
+@DEVICES
+def test_a_call_that_fails_leaves_nothing_behind(device, monkeypatch):
+    """no row or page is kept, and the next call has the results of a new decoder"""
+    paged, other = _make(device, max_requests=2), _make(device, max_requests=2)
+    texts = _texts(61, [8, 5, 6, 3], seed=3)
+    want = other.generate(texts, max_new=4, eos=0)
+    for bad in ([], [1] * 25):  # one that joins late
+        with pytest.raises(ValueError):
+            paged.generate(texts + [bad], max_new=4, eos=0)
+        assert _is_empty(paged)
+    inner, calls = type(paged)._step, []
+
+    def fail_in_the_third(self):
+        calls.append(0)
+        if len(calls) == 3:
+            raise KeyError("in the middle")
+        return inner(self)
+
+    def fail(self, *args):
+        raise KeyError("in a layer")
+
+    with monkeypatch.context() as m:
+        m.setattr(type(paged), "_step", fail_in_the_third)
+        with pytest.raises(KeyError):
+            paged.generate(texts, max_new=4, eos=0, use_graph=False)
+        assert len(calls) == 3 and _is_empty(paged)
+        m.setattr(type(paged), "_layer", fail)
+        for call in (lambda: paged.generate(texts, max_new=4, eos=0), lambda: paged.score(texts), lambda: paged.add([1], texts[:1])):
+            with pytest.raises(KeyError):
+                call()
+            assert _is_empty(paged)
+    got = paged.generate(texts, max_new=4, eos=0)
+    assert [x.labels for x in got] == [x.labels for x in want]
+    for a, b in zip(got, want):
+        assert a.log_probs == pytest.approx(b.log_probs, abs=1e-4)
