@@ -155,16 +155,33 @@ class PagedDecoder:
         if not (0 <= min(labels) and max(labels) < self.emb.shape[0]):  # (here, not by the lookup on the device)
             raise ValueError("paged decoder: labels %i to %i, the vocabulary has %i" % (min(labels), max(labels), self.emb.shape[0]))
 
+    def _check_rows(self, rows: Sequence[int]):
+        if any(not 0 <= r < self.rows for r in rows):
+            raise ValueError("paged decoder: rows %s of %i" % (list(rows), self.rows))
+        if len(set(rows)) != len(rows):
+            raise ValueError("paged decoder: a row twice in %s" % (list(rows),))
+
+    def _empty_rows(self) -> List[int]:
+        return [r for r, have in enumerate(self.lengths.tolist()) if have <= 0]
+
     def add(self, rows: Sequence[int], prompts: Sequence[Sequence[int]]) -> torch.Tensor:
         """
-        New requests in empty rows: their prompts take pages and run through the layers.
+        New requests in empty rows (the host looks at the lengths): their prompts take pages and run through the layers.
 
         :return: [tokens, features] after the last layer, the tokens of the prompts one after another. Rows without room in the pool stay empty (:attr:`lengths`).
         """
         with torch.no_grad(), torch.autocast(self.device.type, enabled=False):
             order = sorted(range(len(rows)), key=lambda i: rows[i])  # (tokens of a call lie in the order of the rows)
+            if len(rows) != len(prompts):
+                raise ValueError("paged decoder: %i prompts for %i rows" % (len(prompts), len(rows)))
+            self._check_rows(rows)
             for prompt in prompts:
                 self._check_prompt(prompt)
+            if not rows:
+                return self.emb.new_zeros(0, self.emb.shape[1])
+            held = set(rows) - set(self._empty_rows())
+            if held:
+                raise ValueError("paged decoder: row %s holds a request" % sorted(held))
             counts = torch.zeros(self.rows, dtype=torch.int32)
             for i in order:
                 counts[rows[i]] = len(prompts[i])
@@ -245,6 +262,7 @@ class PagedDecoder:
 
     def end(self, rows: Sequence[int]):
         """these requests are over: their pages go back to the pool"""
+        self._check_rows(rows)
         done = torch.zeros(self.rows, dtype=torch.bool)
         done[list(rows)] = True
         back = release_pages(self.block_table, self.lengths, done.to(self.device), self.free_pages, self.free_range, page_size=self.page_size)
@@ -254,15 +272,20 @@ class PagedDecoder:
     # ---- what a user calls
 
     def score(self, texts: Sequence[Sequence[int]], *, num_top: int = 0) -> List[ScoredText]:
-        """log probability of every label of each text after its first, the entropy at its position and the best alternatives"""
+        """
+        Log probability of every label of each text after its first, the entropy at its position and the best alternatives. The texts run in rows that hold no request.
+        """
         res: List[ScoredText] = []
-        for at in range(0, len(texts), self.rows):
-            part = texts[at: at + self.rows]
-            rows = list(range(len(part)))
+        empty = self._empty_rows()
+        if texts and not empty:
+            raise RuntimeError("paged decoder: all %i rows hold requests" % self.rows)
+        for at in range(0, len(texts), max(len(empty), 1)):
+            part = texts[at: at + len(empty)]
+            rows = empty[: len(part)]
             x = self.add(rows, part)
             try:
-                lens = self.lengths[: len(part)].tolist()
-                if any(have != len(t) for have, t in zip(lens, part)):
+                lens = self.lengths.tolist()
+                if any(lens[r] != len(t) for r, t in zip(rows, part)):
                     raise RuntimeError("paged decoder: no room for %i texts in %i pages" % (len(part), self.num_pages))
                 targets = torch.tensor([y for t in part for y in list(t[1:]) + [-1]], dtype=torch.int32).to(self.device)
                 with torch.no_grad():
@@ -279,10 +302,13 @@ class PagedDecoder:
     def generate(self, prompts: Sequence[Sequence[int]], *, max_new: int, eos: int, use_graph: Optional[bool] = None) -> List[GeneratedText]:
         """
         The best label after each prompt, and so on until ``eos`` or ``max_new`` labels or the longest length. Prompts beyond the number of rows, or without pages at the moment, wait until
-        others end. One that does not fit the pool alone is an error.
+        others end. One that does not fit the pool alone is an error. They run in rows that hold no request.
         """
         for prompt in prompts:
             self._check_prompt(prompt)
+        empty = self._empty_rows()
+        if prompts and not empty:
+            raise RuntimeError("paged decoder: all %i rows hold requests" % self.rows)
         out = [GeneratedText([], []) for _ in prompts]
         waiting = list(range(len(prompts)))
         running = {}  # row -> prompt
@@ -297,7 +323,7 @@ class PagedDecoder:
         held = set()  # rows that may have pages
         try:
             while waiting or running:
-                free = [r for r in range(self.rows) if r not in running]
+                free = [r for r in empty if r not in running]
                 if waiting and free:
                     rows = free[: len(waiting)]
                     batch = waiting[: len(rows)]

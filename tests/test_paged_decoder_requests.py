@@ -66,3 +66,31 @@ def test_a_call_that_fails_leaves_nothing_behind(device, monkeypatch):
     assert [x.labels for x in got] == [x.labels for x in want]
     for a, b in zip(got, want):
         assert a.log_probs == pytest.approx(b.log_probs, abs=1e-4)
+
+
+@DEVICES
+def test_rows_that_hold_a_request_are_not_taken(device):
+    """add() refuses them; score() and generate() work beside them in the other rows and leave them as they are"""
+    paged, other = _make(device), _make(device)
+    texts = _texts(61, [6, 9, 4, 7], seed=5)
+    paged.add([1], texts[:1])
+    lengths, table = paged.lengths.tolist(), paged.block_table[1, :2].tolist()
+    for rows, err in (([1], "holds"), ([0, 1], "holds"), ([0, 0], "twice"), ([-1, 0], "rows"), ([3, 0], "rows"), ([0], "prompts"), ([], "prompts")):
+        with pytest.raises(ValueError, match=err):
+            paged.add(rows, [[1, 2]] * (len(rows) if "prompts" not in err else len(rows) + 1))
+        assert paged.lengths.tolist() == lengths
+    for bad in ([-1], [3], [0, 7]):
+        with pytest.raises(ValueError, match="rows"):
+            paged.end(bad)
+    for a, b in zip(paged.score(texts, num_top=2), other.score(texts, num_top=2)):
+        assert torch.allclose(a.log_probs, b.log_probs, atol=1e-4) and torch.equal(a.top_labels, b.top_labels)
+    for a, b in zip(paged.generate(texts, max_new=5, eos=0), other.generate(texts, max_new=5, eos=0)):
+        assert a.labels == b.labels
+    assert paged.lengths.tolist() == lengths and paged.block_table[1, :2].tolist() == table
+    paged.add([0, 2], texts[1:3])
+    for call in (lambda: paged.score(texts), lambda: paged.generate(texts, max_new=5, eos=0)):
+        with pytest.raises(RuntimeError, match="rows"):
+            call()
+    assert paged.lengths.tolist() == [9, 6, 4]
+    paged.end([2, 0, 1])
+    assert _is_empty(paged) and paged.add([], []).shape[0] == 0
