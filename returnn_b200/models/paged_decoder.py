@@ -164,6 +164,16 @@ class PagedDecoder:
     def _empty_rows(self) -> List[int]:
         return [r for r, have in enumerate(self.lengths.tolist()) if have <= 0]
 
+    def _that_fit(self, texts: Sequence[Sequence[int]]) -> int:
+        """:return: how many of these, from the first on, have room in the pool together (the host looks at the range of free pages)"""
+        head, tail = self.free_range.tolist()
+        room = tail - head
+        for n, text in enumerate(texts):
+            room -= -(-len(text) // self.page_size)
+            if room < 0:
+                return n
+        return len(texts)
+
     def add(self, rows: Sequence[int], prompts: Sequence[Sequence[int]]) -> torch.Tensor:
         """
         New requests in empty rows (the host looks at the lengths): their prompts take pages and run through the layers.
@@ -282,11 +292,10 @@ class PagedDecoder:
         for at in range(0, len(texts), max(len(empty), 1)):
             part = texts[at: at + len(empty)]
             rows = empty[: len(part)]
+            if self._that_fit(part) < len(part):
+                raise RuntimeError("paged decoder: no room for %i texts in %i pages" % (len(part), self.num_pages))
             x = self.add(rows, part)
             try:
-                lens = self.lengths.tolist()
-                if any(lens[r] != len(t) for r, t in zip(rows, part)):
-                    raise RuntimeError("paged decoder: no room for %i texts in %i pages" % (len(part), self.num_pages))
                 targets = torch.tensor([y for t in part for y in list(t[1:]) + [-1]], dtype=torch.int32).to(self.device)
                 with torch.no_grad():
                     r = token_log_probs(self._logits(x), targets, entropy=True, num_top=num_top)
@@ -306,6 +315,8 @@ class PagedDecoder:
         """
         for prompt in prompts:
             self._check_prompt(prompt)
+            if len(prompt) > self.num_pages * self.page_size:
+                raise RuntimeError("paged decoder: a prompt of %i labels does not fit %i pages" % (len(prompt), self.num_pages))
         empty = self._empty_rows()
         if prompts and not empty:
             raise RuntimeError("paged decoder: all %i rows hold requests" % self.rows)
@@ -324,20 +335,18 @@ class PagedDecoder:
         try:
             while waiting or running:
                 free = [r for r in empty if r not in running]
-                if waiting and free:
-                    rows = free[: len(waiting)]
-                    batch = waiting[: len(rows)]
+                batch = waiting[: len(free)]
+                batch = batch[: self._that_fit([prompts[i] for i in batch])] if batch else batch
+                if batch:
+                    rows = free[: len(batch)]
+                    del waiting[: len(batch)]
                     held.update(rows)
                     x = self.add(rows, [prompts[i] for i in batch])
-                    have = self.lengths.tolist()
                     ends = torch.tensor([len(prompts[i]) for i in batch]).cumsum(0) - 1
                     with torch.no_grad():
                         best = token_log_probs(self._logits(x[ends.to(self.device)]), self._ignored[: len(batch)], num_top=1)
                     over = []
                     for r, i, label, lp in zip(rows, batch, best.top_labels[:, 0].tolist(), best.top_log_probs[:, 0].tolist()):
-                        if not have[r]:  # the pool was empty: again later
-                            continue
-                        waiting.remove(i)
                         if max_new > 0 and take(i, label, lp):
                             running[r], last[r] = i, label
                         else:
@@ -345,8 +354,8 @@ class PagedDecoder:
                     if over:
                         self.end(over)
                         held.difference_update(over)
-                    elif not running:
-                        raise RuntimeError("paged decoder: prompts of %s labels do not fit %i pages" % ([len(prompts[i]) for i in batch], self.num_pages))
+                elif not running:
+                    raise RuntimeError("paged decoder: a prompt of %i labels does not fit what is free of %i pages" % (len(prompts[waiting[0]]), self.num_pages))
                 if not running:
                     continue
                 active.zero_()

@@ -94,3 +94,26 @@ def test_rows_that_hold_a_request_are_not_taken(device):
     assert paged.lengths.tolist() == [9, 6, 4]
     paged.end([2, 0, 1])
     assert _is_empty(paged) and paged.add([], []).shape[0] == 0
+
+
+@DEVICES
+def test_prompts_that_wait_do_not_run(device, monkeypatch):
+    """whether a prompt has room is known before it goes through the layers"""
+    paged = _make(device, max_requests=3, num_pages=8)
+    texts = _texts(61, [9, 13, 12, 8, 3], seed=6)  # 3, 4, 3, 2 and 1 of the 8 pages
+    want = _make(device).generate(texts, max_new=4, eos=-1)
+    ran, inner = [], type(paged).add
+
+    def add(self, rows, prompts):
+        ran.extend(prompts)
+        return inner(self, rows, prompts)
+
+    monkeypatch.setattr(type(paged), "add", add)
+    got = paged.generate(texts, max_new=4, eos=-1)
+    assert ran == texts and [x.labels for x in got] == [x.labels for x in want] and _is_empty(paged)
+    del ran[:]
+    small = _make(device, num_pages=2)
+    for call in (lambda: small.generate([texts[4], texts[0]], max_new=2, eos=-1), lambda: small.score([texts[4], texts[0]])):
+        with pytest.raises(RuntimeError, match="2 pages"):
+            call()
+        assert _is_empty(small) and not ran
