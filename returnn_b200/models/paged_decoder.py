@@ -311,7 +311,8 @@ class PagedDecoder:
     def generate(self, prompts: Sequence[Sequence[int]], *, max_new: int, eos: int, use_graph: Optional[bool] = None) -> List[GeneratedText]:
         """
         The best label after each prompt, and so on until ``eos`` or ``max_new`` labels or the longest length. Prompts beyond the number of rows, or without pages at the moment, wait until
-        others end. One that does not fit the pool alone is an error. They run in rows that hold no request.
+        others end. Where none of the running ones can go on for want of a page, the one that began last gives its pages up; it waits, and its prompt and labels so far run through the layers
+        again. One that does not fit the pool alone is an error. They run in rows that hold no request.
         """
         for prompt in prompts:
             self._check_prompt(prompt)
@@ -322,7 +323,8 @@ class PagedDecoder:
             raise RuntimeError("paged decoder: all %i rows hold requests" % self.rows)
         out = [GeneratedText([], []) for _ in prompts]
         waiting = list(range(len(prompts)))
-        running = {}  # row -> prompt
+        running = {}  # row -> prompt, in the order in which they began
+        stuck: List[int] = []  # rows that found no page in the last step; others join when there are none
         last, active = torch.zeros(self.rows, dtype=torch.int64), torch.zeros(self.rows, dtype=torch.int32)
 
         def take(i: int, label: int, log_prob: float) -> bool:
@@ -335,14 +337,15 @@ class PagedDecoder:
         try:
             while waiting or running:
                 free = [r for r in empty if r not in running]
-                batch = waiting[: len(free)]
-                batch = batch[: self._that_fit([prompts[i] for i in batch])] if batch else batch
+                batch = waiting[: len(free)] if not stuck else []
+                text = {i: list(prompts[i]) + out[i].labels for i in batch}
+                batch = batch[: self._that_fit([text[i] for i in batch])] if batch else batch
                 if batch:
                     rows = free[: len(batch)]
                     del waiting[: len(batch)]
                     held.update(rows)
-                    x = self.add(rows, [prompts[i] for i in batch])
-                    ends = torch.tensor([len(prompts[i]) for i in batch]).cumsum(0) - 1
+                    x = self.add(rows, [text[i] for i in batch])
+                    ends = torch.tensor([len(text[i]) for i in batch]).cumsum(0) - 1
                     with torch.no_grad():
                         best = token_log_probs(self._logits(x[ends.to(self.device)]), self._ignored[: len(batch)], num_top=1)
                     over = []
@@ -355,7 +358,8 @@ class PagedDecoder:
                         self.end(over)
                         held.difference_update(over)
                 elif not running:
-                    raise RuntimeError("paged decoder: a prompt of %i labels does not fit what is free of %i pages" % (len(prompts[waiting[0]]), self.num_pages))
+                    i = waiting[0]
+                    raise RuntimeError("paged decoder: a prompt of %i labels and %i more do not fit what is free of %i pages" % (len(prompts[i]), len(out[i].labels), self.num_pages))
                 if not running:
                     continue
                 active.zero_()
@@ -373,8 +377,11 @@ class PagedDecoder:
                         last[r] = label
                     else:
                         over.append(r)
-                if stuck and len(stuck) == len(running):
-                    raise RuntimeError("paged decoder: %i running requests and no free page of %i" % (len(stuck), self.num_pages))
+                if len(stuck) == len(running):
+                    last_row = list(running)[-1]
+                    waiting.insert(0, running[last_row])
+                    over.append(last_row)
+                    stuck.remove(last_row)
                 for r in over:
                     del running[r]
                 if over:

@@ -16,6 +16,20 @@ def _make(device="cpu", kind="normed", **opts):
     return PagedDecoder(model, **{**dict(max_requests=3, max_len=24, page_size=4), **opts})
 
 
+def _same(got, want, device):
+    """
+    The same labels and log probabilities: sums of 32 to 140 products in fp32 through two layers, in another order. On the GPU prompts and steps take other kernels, each within 1e-3 of the
+    model's call; two labels may be as good as each other there, and what follows is then another text.
+    """
+    tol = 1e-4 if device == "cpu" else 2e-3
+    for a, b, x, y in zip(got.labels, want.labels, got.log_probs, want.log_probs):
+        assert abs(x - y) <= tol * (1 + abs(y))
+        if a != b:
+            assert device != "cpu"
+            return
+    assert len(got.labels) == len(want.labels)
+
+
 def _is_empty(paged):
     return not paged.lengths.any() and int(paged.free_range[1] - paged.free_range[0]) == paged.num_pages
 
@@ -63,9 +77,8 @@ def test_a_call_that_fails_leaves_nothing_behind(device, monkeypatch):
                 call()
             assert _is_empty(paged)
     got = paged.generate(texts, max_new=4, eos=0)
-    assert [x.labels for x in got] == [x.labels for x in want]
     for a, b in zip(got, want):
-        assert a.log_probs == pytest.approx(b.log_probs, abs=1e-4)
+        _same(a, b, device)
 
 
 @DEVICES
@@ -83,9 +96,10 @@ def test_rows_that_hold_a_request_are_not_taken(device):
         with pytest.raises(ValueError, match="rows"):
             paged.end(bad)
     for a, b in zip(paged.score(texts, num_top=2), other.score(texts, num_top=2)):
-        assert torch.allclose(a.log_probs, b.log_probs, atol=1e-4) and torch.equal(a.top_labels, b.top_labels)
+        tol = 1e-4 if device == "cpu" else 2e-3
+        assert torch.allclose(a.log_probs, b.log_probs, atol=tol, rtol=tol) and torch.allclose(a.top_log_probs, b.top_log_probs, atol=tol, rtol=tol)
     for a, b in zip(paged.generate(texts, max_new=5, eos=0), other.generate(texts, max_new=5, eos=0)):
-        assert a.labels == b.labels
+        _same(a, b, device)
     assert paged.lengths.tolist() == lengths and paged.block_table[1, :2].tolist() == table
     paged.add([0, 2], texts[1:3])
     for call in (lambda: paged.score(texts), lambda: paged.generate(texts, max_new=5, eos=0)):
@@ -110,10 +124,34 @@ def test_prompts_that_wait_do_not_run(device, monkeypatch):
 
     monkeypatch.setattr(type(paged), "add", add)
     got = paged.generate(texts, max_new=4, eos=-1)
-    assert ran == texts and [x.labels for x in got] == [x.labels for x in want] and _is_empty(paged)
+    assert ran == texts and _is_empty(paged)
+    for a, b in zip(got, want):
+        _same(a, b, device)
     del ran[:]
     small = _make(device, num_pages=2)
     for call in (lambda: small.generate([texts[4], texts[0]], max_new=2, eos=-1), lambda: small.score([texts[4], texts[0]])):
         with pytest.raises(RuntimeError, match="2 pages"):
             call()
         assert _is_empty(small) and not ran
+
+
+@DEVICES
+@pytest.mark.parametrize("lens,pages,max_new", [([8, 8], 6, 14), ([8, 7, 5], 6, 16), ([4, 4, 4, 4, 4], 6, 20), ([1, 1, 1], 3, 11), ([20, 3, 3], 6, 4)])
+def test_requests_that_outgrow_the_pool_together(device, lens, pages, max_new):
+    """each fits the pool alone: the one that began last gives its pages up and goes on later, with the results of a run of its own"""
+    paged = _make(device, num_pages=pages)
+    texts = _texts(61, lens, seed=7)
+    got = paged.generate(texts, max_new=max_new, eos=-1)
+    assert _is_empty(paged)
+    for text, res in zip(texts, got):
+        (alone,) = _make(device).generate([text], max_new=max_new, eos=-1)
+        assert len(res.labels) == len(alone.labels) == max_new
+        _same(res, alone, device)
+
+
+@DEVICES
+def test_a_request_that_outgrows_the_pool_alone(device):
+    paged = _make(device, num_pages=2)
+    with pytest.raises(RuntimeError, match="2 pages"):
+        paged.generate(_texts(61, [3, 5], seed=8), max_new=10, eos=-1)
+    assert _is_empty(paged)
