@@ -145,7 +145,8 @@ class PagedDecoder:
         return x + F.linear(h, lay["ff2"][0].t(), lay["ff2"][1])
 
     def _logits(self, x: torch.Tensor) -> torch.Tensor:
-        return F.linear(_apply_norm(x, self.final_norm), self.logits_w.t(), self.logits_b)
+        with torch.autocast(self.device.type, enabled=False):
+            return F.linear(_apply_norm(x, self.final_norm), self.logits_w.t(), self.logits_b)
 
     # ---- requests
 

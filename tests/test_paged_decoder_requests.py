@@ -155,3 +155,16 @@ def test_a_request_that_outgrows_the_pool_alone(device):
     with pytest.raises(RuntimeError, match="2 pages"):
         paged.generate(_texts(61, [3, 5], seed=8), max_new=10, eos=-1)
     assert _is_empty(paged)
+
+
+@DEVICES
+def test_the_callers_autocast_changes_nothing(device):
+    """the types are those of the decoder: the same bits"""
+    paged = _make(device)
+    texts = _texts(61, [6, 9, 4], seed=9)
+    want, want_texts = paged.score(texts, num_top=2), paged.generate(texts, max_new=3, eos=-1)
+    with torch.autocast(device, dtype=torch.bfloat16):
+        got, got_texts = paged.score(texts, num_top=2), paged.generate(texts, max_new=3, eos=-1)
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) and x.dtype == y.dtype for x, y in zip(a, b))
+    assert got_texts == want_texts
