@@ -5,7 +5,13 @@ generation over a paged key / value cache.
 Keys and values of all running requests lie in pages of ``page_size`` tokens, one pool per layer under one block table; a request takes pages as it grows and gives them back when
 it ends (:mod:`returnn_b200.ops.paged`). A step of all running requests is a fixed sequence of kernels on fixed addresses: pages and slots of the new tokens, per layer the
 projection, norm and rotation into the cache, attention over the pages, feed-forward; the output layer and its best label with its log probability. On the GPU it is captured
-once as a CUDA graph; which rows take part is a tensor, so that requests join and leave between replays. The host looks at the labels once per step.
+once as a CUDA graph; which rows take part is a tensor, so that requests join and leave between replays. Between two steps the host reads the results of the first.
+
+A serving loop of its own, where :meth:`PagedDecoder.generate` is not what is wanted::
+
+    x = paged.add([row], [prompt])                       # the prompt runs through the layers; paged.logits(x[-1:]) is about its next label
+    labels, log_probs, rows, granted = paged.step({row: label, ...})
+    paged.end([row])
 
 New requests run through the layers as packed rows, their keys and values going to their pages on the way, with ordinary causal attention inside each prompt.
 
@@ -13,7 +19,7 @@ The reference decodes by the step interface over states that grow by concatenati
 """
 
 from __future__ import annotations
-from typing import List, NamedTuple, Optional, Sequence
+from typing import Dict, List, Mapping, NamedTuple, Optional, Sequence
 import torch
 import torch.nn.functional as F
 
@@ -144,7 +150,8 @@ class PagedDecoder:
             h = act(a) * gate(g)
         return x + F.linear(h, lay["ff2"][0].t(), lay["ff2"][1])
 
-    def _logits(self, x: torch.Tensor) -> torch.Tensor:
+    def logits(self, x: torch.Tensor) -> torch.Tensor:
+        """output layer for features [tokens, features] that :meth:`add` returned"""
         with torch.autocast(self.device.type, enabled=False):
             return F.linear(_apply_norm(x, self.final_norm), self.logits_w.t(), self.logits_b)
 
@@ -153,6 +160,9 @@ class PagedDecoder:
     def _check_prompt(self, labels: Sequence[int]):
         if not 0 < len(labels) <= self.max_len:
             raise ValueError("paged decoder: a prompt of %i labels (1 to %i)" % (len(labels), self.max_len))
+        self._check_labels(labels)
+
+    def _check_labels(self, labels: Sequence[int]):
         if not (0 <= min(labels) and max(labels) < self.emb.shape[0]):  # (here, not by the lookup on the device)
             raise ValueError("paged decoder: labels %i to %i, the vocabulary has %i" % (min(labels), max(labels), self.emb.shape[0]))
 
@@ -241,15 +251,27 @@ class PagedDecoder:
         x = self._embed(self._last.index_select(0, row), new.positions)
         for lay in self.layers:
             x = self._layer(lay, x, new, lambda la, q, k, v: paged_attention(q, la["k"], la["v"], table, lengths).flatten(1))
-        best = token_log_probs(self._logits(x), self._ignored, num_top=1)
+        best = token_log_probs(self.logits(x), self._ignored, num_top=1)
         return best.top_labels[:, 0], best.top_log_probs[:, 0], new.requests, new.granted
 
-    def step(self, *, use_graph: Optional[bool] = None):
+    def step(self, labels: Optional[Mapping[int, int]] = None, *, use_graph: Optional[bool] = None):
         """
-        One more token for every row of :attr:`_active`, which continue with their :attr:`_last` label.
+        One more token for some rows.
 
-        :return: best label, its log probability and row of each (rows in ascending order, -1 behind the last), and whether each row was granted its page
+        :param labels: row -> label that it continues with, the last one of its prompt or the one that the step before found; the row may be empty.
+            None: the rows and labels of the call before, without those that have ended.
+        :return: best label, its log probability and row of each (rows in ascending order, -1 behind the last), and for each row of the decoder whether it was granted its page.
+            The next step overwrites them. A row without a page stays as it was, and can take the same label again when another request has ended.
         """
+        if labels is not None:
+            self._check_rows(list(labels))
+            if labels:
+                self._check_labels(list(labels.values()))
+            active, last = torch.zeros(self.rows, dtype=torch.int32), torch.zeros(self.rows, dtype=torch.int64)
+            for row, label in labels.items():
+                active[row], last[row] = 1, label
+            self._active.copy_(active)
+            self._last.copy_(last)
         if use_graph is None:
             use_graph = self.device.type == "cuda"
         with torch.no_grad(), torch.autocast(self.device.type, enabled=False):
@@ -276,7 +298,9 @@ class PagedDecoder:
         self._check_rows(rows)
         done = torch.zeros(self.rows, dtype=torch.bool)
         done[list(rows)] = True
-        back = release_pages(self.block_table, self.lengths, done.to(self.device), self.free_pages, self.free_range, page_size=self.page_size)
+        done = done.to(self.device)
+        self._active.masked_fill_(done, 0)
+        back = release_pages(self.block_table, self.lengths, done, self.free_pages, self.free_range, page_size=self.page_size)
         self.lengths.copy_(back.lengths)
         self.free_range.copy_(back.free_range)
 
@@ -299,7 +323,7 @@ class PagedDecoder:
             try:
                 targets = torch.tensor([y for t in part for y in list(t[1:]) + [-1]], dtype=torch.int32).to(self.device)
                 with torch.no_grad():
-                    r = token_log_probs(self._logits(x), targets, entropy=True, num_top=num_top)
+                    r = token_log_probs(self.logits(x), targets, entropy=True, num_top=num_top)
             finally:
                 self.end(rows)
             first = 0
@@ -326,7 +350,7 @@ class PagedDecoder:
         waiting = list(range(len(prompts)))
         running = {}  # row -> prompt, in the order in which they began
         stuck: List[int] = []  # rows that found no page in the last step; others join when there are none
-        last, active = torch.zeros(self.rows, dtype=torch.int64), torch.zeros(self.rows, dtype=torch.int32)
+        last: Dict[int, int] = {}  # label that a row continues with
 
         def take(i: int, label: int, log_prob: float) -> bool:
             """:return: whether the request goes on"""
@@ -348,7 +372,7 @@ class PagedDecoder:
                     x = self.add(rows, [text[i] for i in batch])
                     ends = torch.tensor([len(text[i]) for i in batch]).cumsum(0) - 1
                     with torch.no_grad():
-                        best = token_log_probs(self._logits(x[ends.to(self.device)]), self._ignored[: len(batch)], num_top=1)
+                        best = token_log_probs(self.logits(x[ends.to(self.device)]), self._ignored[: len(batch)], num_top=1)
                     over = []
                     for r, i, label, lp in zip(rows, batch, best.top_labels[:, 0].tolist(), best.top_log_probs[:, 0].tolist()):
                         if max_new > 0 and take(i, label, lp):
@@ -363,11 +387,7 @@ class PagedDecoder:
                     raise RuntimeError("paged decoder: a prompt of %i labels and %i more do not fit what is free of %i pages" % (len(prompts[i]), len(out[i].labels), self.num_pages))
                 if not running:
                     continue
-                active.zero_()
-                active[list(running)] = 1
-                self._active.copy_(active)
-                self._last.copy_(last)
-                labels, log_probs, requests, granted = self.step(use_graph=use_graph)
+                labels, log_probs, requests, granted = self.step({r: last[r] for r in running}, use_graph=use_graph)
                 over, stuck = [], []
                 for r, label, lp, ok in zip(requests.tolist(), labels.tolist(), log_probs.tolist(), granted[requests.clamp(min=0).long()].tolist()):
                     if r < 0:

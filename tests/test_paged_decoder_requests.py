@@ -168,3 +168,45 @@ def test_the_callers_autocast_changes_nothing(device):
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) and x.dtype == y.dtype for x, y in zip(a, b))
     assert got_texts == want_texts
+
+
+@DEVICES
+def test_serving_by_public_calls(device):
+    """add, logits, step and end, with requests that join and leave, against generate()"""
+    paged = _make(device, kind="rotary")
+    texts = _texts(61, [6, 9, 1, 4], seed=10)
+    want = _make(device, kind="rotary").generate(texts, max_new=4, eos=-1)
+    out, row_of = {}, {}
+
+    def join(i, row):
+        x = paged.add([row], [texts[i]])
+        label = int(paged.logits(x[-1:])[0].argmax())
+        out[i], row_of[i] = [label], row
+
+    join(1, 2)
+    join(0, 0)
+    waiting = [2, 3]
+    while row_of:
+        labels, log_probs, rows, granted = paged.step({r: out[i][-1] for i, r in row_of.items()})
+        assert rows.tolist()[: len(row_of)] == sorted(row_of.values()) and granted[list(row_of.values())].all()
+        by_row = {r: (a, p) for r, a, p in zip(rows.tolist(), labels.tolist(), log_probs.tolist()) if r >= 0}
+        for i, r in list(row_of.items()):
+            out[i].append(by_row[r][0])
+            if len(out[i]) == 4:
+                del row_of[i]
+                paged.end([r])
+        if waiting and len(row_of) < 3:
+            join(waiting[0], ({0, 1, 2} - set(row_of.values())).pop())
+            del waiting[0]
+    assert _is_empty(paged)
+    for i, res in enumerate(want):
+        assert out[i] == res.labels
+    # rows that have ended do not go on; a request can begin with a step
+    assert paged.step()[2].tolist() == [-1] * 3 and _is_empty(paged)
+    paged.add([1], [texts[0][:-1]])
+    labels, _, rows, _ = paged.step({1: texts[0][-1], 0: texts[2][0]})
+    assert rows.tolist() == [0, 1, -1] and labels.tolist()[:2] == [want[2].labels[0], want[0].labels[0]] and paged.lengths.tolist() == [1, 6, 0]
+    for bad, err in (({3: 1}, "rows"), ({-1: 1}, "rows"), ({0: 61}, "vocabulary"), ({0: -1}, "vocabulary")):
+        with pytest.raises(ValueError, match=err):
+            paged.step(bad)
+    assert paged.lengths.tolist() == [1, 6, 0]
