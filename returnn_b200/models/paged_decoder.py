@@ -78,7 +78,7 @@ class PagedDecoder:
             fn = decoder.pos_enc
             if getattr(fn, "func", fn) is not sinusoidal_positional_encoding:
                 raise TypeError("paged decoder: positional encoding %r is not covered" % (fn,))
-            steps = Dim(max_len, name="steps")
+            steps = Dim(blocks * page_size, name="steps")  # (all positions that have a place)
             self.pos_table = cast(fn(spatial_dim=steps, device=str(self.device)).copy_transpose([steps, decoder.model_dim]).raw_tensor)
         self.layers = []
         for layer in decoder.layers:
@@ -127,7 +127,7 @@ class PagedDecoder:
         if self.emb_scale != 1.0:
             x = x * self.emb_scale
         if self.pos_table is not None:
-            x = x + self.pos_table.index_select(0, positions.long().clamp(max=self.max_len - 1))
+            x = x + self.pos_table.index_select(0, positions.long().clamp(max=self.pos_table.shape[0] - 1))
         return x
 
     def _layer(self, lay, x: torch.Tensor, new, attend) -> torch.Tensor:

@@ -210,3 +210,22 @@ def test_serving_by_public_calls(device):
         with pytest.raises(ValueError, match=err):
             paged.step(bad)
     assert paged.lengths.tolist() == [1, 6, 0]
+
+
+@DEVICES
+@pytest.mark.parametrize("kind", ["sinusoidal", "rotary"])
+def test_positions_in_the_last_page(device, kind):
+    """a page may reach beyond the longest length: positions there are their own, and past the page no token is granted"""
+    from test_paged_decoder import _rf_logits
+
+    paged, model = _make(device, kind=kind, max_len=6), _decoder(kind, dim=32 if device == "cpu" else 128, device=device)
+    text = _texts(61, [8], seed=11)[0]
+    paged.add([1], [text[:6]])
+    with torch.no_grad():
+        want = torch.log_softmax(_rf_logits(model, text, device).double(), -1)
+    for n in (6, 7):
+        _, log_probs, rows, granted = paged.step({1: text[n]})
+        assert rows.tolist() == [1, -1, -1] and granted.all()
+        assert abs(float(log_probs[0]) - float(want[n].max())) <= (1e-4 if device == "cpu" else 1e-3) * (1 + abs(float(want[n].max())))
+    _, _, rows, granted = paged.step({1: 5})
+    assert granted.tolist() == [True, False, True] and paged.lengths.tolist() == [0, 8, 0]
