@@ -26,6 +26,7 @@ import torch.nn.functional as F
 from ..ops import attention as _att
 from ..ops.norm_rope import norm_rope_to_cache, rope_frequencies
 from ..ops.paged import append_tokens, paged_attention, release_pages
+from ..ops.status import KernelWaitTimeout, StatusPoller
 from ..ops.token_log_probs import token_log_probs
 from .decode_graph import _lin, _norm, _apply_norm, _activation
 
@@ -119,6 +120,7 @@ class PagedDecoder:
         self._ignored = torch.full((max_requests,), -1, **i32)
         self._graph = None
         self._step_out = None
+        self._status = StatusPoller(self.device)
 
     # ---- the layers
 
@@ -262,6 +264,7 @@ class PagedDecoder:
             None: the rows and labels of the call before, without those that have ended.
         :return: best label, its log probability and row of each (rows in ascending order, -1 behind the last), and for each row of the decoder whether it was granted its page.
             The next step overwrites them. A row without a page stays as it was, and can take the same label again when another request has ended.
+            A kernel of the step that gave up a wait is an error (:class:`returnn_b200.ops.status.KernelWaitTimeout`) in the next call.
         """
         if labels is not None:
             self._check_rows(list(labels))
@@ -276,7 +279,9 @@ class PagedDecoder:
             use_graph = self.device.type == "cuda"
         with torch.no_grad(), torch.autocast(self.device.type, enabled=False):
             if not use_graph:
-                return self._step()
+                out = self._step()
+                self._look_at_status()
+                return out
             if self._graph is None:
                 # lazy initialisation outside the capture, with no row taking part
                 active = self._active.clone()
@@ -291,7 +296,18 @@ class PagedDecoder:
                 with torch.cuda.graph(self._graph):
                     self._step_out = self._step()
             self._graph.replay()
+            self._look_at_status()
             return self._step_out
+
+    def _look_at_status(self, wait: bool = False):
+        """whether a kernel gave up a wait, in what was queued before the last call, or in all so far"""
+        try:
+            self._status.step(where="paged decoder")
+            if wait:
+                self._status.flush(where="paged decoder")
+        except KernelWaitTimeout:
+            self._status = StatusPoller(self.device)  # (copies still under way show the same)
+            raise
 
     def end(self, rows: Sequence[int]):
         """these requests are over: their pages go back to the pool"""
@@ -331,6 +347,7 @@ class PagedDecoder:
                 cut = slice(first, first + len(t) - 1)
                 res.append(ScoredText(r.log_probs[cut], r.entropy[cut], r.top_labels[cut] if num_top else None, r.top_log_probs[cut] if num_top else None))
                 first += len(t)
+        self._look_at_status(wait=True)
         return res
 
     def generate(self, prompts: Sequence[Sequence[int]], *, max_new: int, eos: int, use_graph: Optional[bool] = None) -> List[GeneratedText]:
@@ -408,6 +425,7 @@ class PagedDecoder:
                 if over:
                     self.end(over)
                     held.difference_update(over)
+            self._look_at_status(wait=True)
         finally:
             if held:
                 self.end(sorted(held))

@@ -15,7 +15,7 @@ from __future__ import annotations
 from typing import Callable, Dict, List, Optional, Tuple
 import torch
 
-SLOT_GEMM = 0  # tcgen05 GEMM family, attention GEMMs, persistent LSTM, native encoder executor
+SLOT_GEMM = 0  # tcgen05 GEMM family, attention GEMMs, attention over a paged cache, persistent LSTM, native encoder executor
 SLOT_ALLREDUCE = 1  # fused gradient all-reduce
 SLOT_PARAM_AVG = 2  # fused AdamW + parameter averaging
 SLOT_SMALL_REDUCE = 3  # small-vector all-reduce (batch-norm statistics)
@@ -63,6 +63,8 @@ def register_describer(slot: int, fn: Callable[[int], str]):
 
 
 def _describe_gemm(v: int) -> str:
+    if (v >> 24) & 0xFF == 9:
+        return "attention over a paged cache: bounded wait of a %s warp ran out" % ("loading" if v & 0xFFFFFF == 1 else "multiplying")
     return "tcgen05 GEMM / persistent LSTM: bounded wait ran out (role %i, position %i)" % ((v >> 24) & 0xFF, v & 0xFFFFFF)
 
 

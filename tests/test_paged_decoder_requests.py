@@ -229,3 +229,27 @@ def test_positions_in_the_last_page(device, kind):
         assert abs(float(log_probs[0]) - float(want[n].max())) <= (1e-4 if device == "cpu" else 1e-3) * (1 + abs(float(want[n].max())))
     _, _, rows, granted = paged.step({1: 5})
     assert granted.tolist() == [True, False, True] and paged.lengths.tolist() == [0, 8, 0]
+
+
+def test_a_wait_that_ran_out_is_named():
+    from returnn_b200.ops import status
+
+    assert "paged cache" in status.describe(status.SLOT_GEMM, 9 << 24 | 1) and "GEMM" not in status.describe(status.SLOT_GEMM, 9 << 24 | 1)
+    assert "GEMM" in status.describe(status.SLOT_GEMM, 3 << 24 | 1)
+
+
+@gpu
+def test_a_wait_that_ran_out_is_an_error():
+    """what a kernel that gave up leaves on the status board (written here by the host): no labels or scores that are not valid are returned"""
+    from returnn_b200.ops import status
+
+    paged = _make("cuda")
+    texts = _texts(61, [6, 9], seed=12)
+    want = paged.generate(texts, max_new=4, eos=-1)
+    word = status.word("cuda", status.SLOT_GEMM)
+    for call in (lambda: paged.generate(texts, max_new=4, eos=-1), lambda: paged.score(texts), lambda: [paged.step({}) for _ in range(2)]):
+        word.fill_(9 << 24 | 1)
+        with pytest.raises(status.KernelWaitTimeout, match="paged cache"):
+            call()
+        assert _is_empty(paged) and not int(word)
+    assert [x.labels for x in paged.generate(texts, max_new=4, eos=-1)] == [x.labels for x in want]
