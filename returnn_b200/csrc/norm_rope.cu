@@ -10,8 +10,8 @@
 // Rows are read once and written once. A row of D features sits in the next power of two of D / 8 lanes, 8 features a lane, chosen so that both features of a pair
 // are the lane's own: 8 in a row for pairs (2i, 2i + 1), 4 of each half for pairs (i, i + R / 2). The mean is a few shuffles. Head dims, rotated parts and
 // alignments that do not fit this take a warp per row with single elements.
-// Measured, both passes with the norm: 25000 x 16 heads of 64, bf16, 256 MB, 61.8 us (4.1 TB/s; a copy of as many bytes takes 42), bound by the instructions of a row of 128
-// bytes; 8191 x 40 of 128, fp32, 839 MB, 138.5 us (6.1 TB/s, what the memory gives).
+// Measured, both passes with the norm: 25000 x 16 heads of 64, bf16, 256 MB, 62 us (4.1 TB/s; a copy of as many bytes takes 42), bound by latency: 57 to 65 % of the issue
+// slots and 28 to 40 % of the memory's rate are in use, with 45 % of the warps that an SM holds; 8191 x 40 of 128, fp32, 839 MB, 138.5 us (6.1 TB/s, what the memory gives).
 #include "packed_f32.cuh"
 #include <algorithm>
 #include <cstdlib>

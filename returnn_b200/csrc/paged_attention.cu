@@ -1,6 +1,7 @@
 // Attention of one new token per request over a paged key / value cache.
 //   out[i, h, :] = softmax_t(scale q[i, h, :] . K[t, h / G, :]) V[t, h / G, :],  t < len_i; token t lies in page table[i][t / P] at place t % P
-// G = query heads per key head. A request without tokens gets zeros. Every key and value is read once; the pass is bound by that.
+// G = query heads per key head. A request without tokens gets zeros. Keys and values are read once for every 32 (bf16) or 8 (fp32) query heads of their key head; with up to
+// that many in bf16, and up to 4 in fp32, the pass is bound by that where requests are long.
 //
 // Split: the work is a list of tiles, ordered by (request, group of units, tile); each CTA takes an equally costly stretch of the list, whatever the lengths
 // of the requests are (a long document next to short ones, few requests of many tokens). A stretch that holds all tiles of a (request, group)
@@ -18,9 +19,10 @@
 // rows 0..7 are 8 query heads with the upper 16 bits of the weights, rows 8..15 the same heads with what is left of them in bf16. Their sum weighs the
 // values with 16 bits of mantissa at no further instruction; weights of 8 bits would add an error as large as the rounding of the result.
 // fp32: products by fused multiply-adds, a kernel for 1, 2, 4 and 8 heads of a unit (14 requests, 56340 tokens, D 128, 4 on each of 8 key heads: 88 us; with one kernel and the heads
-// counted at run time 169).
-// Measured (D 128, 4 query heads on each of 8 key heads, bf16): 64 requests of 122637 tokens together, 502 MB, 85 us (5.9 TB/s); two of 76484 and 131072, 850 MB, 132 us
-// (6.4 TB/s). Small calls are the launches and the chain of length, page, token, product and join: one request of 1000 tokens, fp32, D 64, 8.2 us.
+// counted at run time 169). With 8 or more heads on a key head it is latency that sets the pace: 16 on one of 128, 14 x 4024 tokens, 45 us where one read of the cache takes 9 and
+// the multiply-adds 6; 32 % of the issue slots, 18 % of the multiply-add units' and 30 % of the shared memory's rate are in use, with 12 warps on an SM.
+// Measured (D 128, 4 query heads on each of 8 key heads, bf16): 64 requests of 122637 tokens together, 502 MB, 84 us (6.0 TB/s); two of 76484 and 131072, 850 MB, 132 us
+// (6.4 TB/s). Small calls are at present two launches and a chain of length, page, token, product and join: one request of 1000 tokens, fp32, D 64, 8.2 us.
 #include "packed_f32.cuh"
 #include "tcgen05.cuh"
 #include <algorithm>

@@ -33,7 +33,9 @@ _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes
 
 
 class AppendedTokens(NamedTuple):
-    """what :func:`append_tokens` returns"""
+    """
+    what :func:`append_tokens` returns. On the GPU the tensors may share one allocation: one that is kept keeps the memory of all (copy it to keep it alone).
+    """
 
     slots: torch.Tensor  # [max_tokens] int32, page * page size + place in the page; -1: no place (request not granted, or room without a token)
     positions: torch.Tensor  # [max_tokens] int32 position in the request; 0 in room without a token
@@ -45,7 +47,7 @@ class AppendedTokens(NamedTuple):
 
 
 class ReleasedPages(NamedTuple):
-    """what :func:`release_pages` returns"""
+    """what :func:`release_pages` returns; see :class:`AppendedTokens` about their memory"""
 
     lengths: torch.Tensor  # [requests] int32, 0 where finished
     free_range: torch.Tensor  # [2] int64
@@ -149,6 +151,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     scale: Optional[float] = None) -> torch.Tensor:
     """
     Attention of one query per request over its cached tokens (the newest among them: ``lengths`` counts it), without gradient.
+
+    The waits in the kernel are bounded. One that runs out leaves its code on the status board (:mod:`returnn_b200.ops.status`), and the result is not valid: programs of their own
+    look at the board with :class:`returnn_b200.ops.status.StatusPoller` or :func:`returnn_b200.ops.status.check_now`.
 
     :param q: [requests, heads, D] bf16 or fp32, unit stride over D
     :param k_cache: [pages, key heads, page size, D] of the same type, D a multiple of 8 up to 256; any strides with unit stride over D

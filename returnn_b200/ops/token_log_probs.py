@@ -23,7 +23,9 @@ MAX_TOP = 32
 
 
 class TokenLogProbs(NamedTuple):
-    """what :func:`token_log_probs` returns; None: not asked for"""
+    """
+    what :func:`token_log_probs` returns; None: not asked for. On the GPU the tensors may share one allocation: one that is kept keeps the memory of all (copy it to keep it alone).
+    """
 
     log_probs: torch.Tensor  # [rows] fp32
     entropy: Optional[torch.Tensor] = None  # [rows] fp32
@@ -79,7 +81,7 @@ class _TokenLogProbsFn(torch.autograd.Function):
 
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, *, entropy: bool = False, num_top: int = 0) -> TokenLogProbs:
     """
-    See the module docstring; differentiable in ``logits`` (through all three results).
+    See the module docstring; differentiable in ``logits`` (through all three results), once.
 
     :param logits: [rows, V] bf16 or fp32, unit stride over V (rows may lie further apart: the first V columns of a padded product)
     :param targets: [rows] int32 or int64
